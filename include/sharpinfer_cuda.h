@@ -510,7 +510,8 @@ si_status si_paged_attention(const si_paged_cache *cache, uint32_t type, const v
  *           x = x - frequency[r] * n;  x = x - presence[r]
  *   bias:   x = x + value of the row's last bias entry for v
  *   mask:   x = -inf when the row has a mask and v's bit in it is 0
- * in FP32, rounded once to `type`. Tokens outside [0, vocab) are ignored. */
+ * in FP32, rounded once to `type`. Tokens outside [0, vocab) are ignored. A list
+ * of count 0 is absent, whatever its other pointers are: none of them is read. */
 typedef struct si_logit_controls {
     const int32_t *history;        /* [history_count]; row r's tokens at history_starts[r] .. [r + 1] */
     const int32_t *history_starts; /* [rows + 1] */

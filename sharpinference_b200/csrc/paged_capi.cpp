@@ -193,7 +193,11 @@ si_status si_process_logits(uint32_t type, const void *logits, int64_t logits_st
     if (logits_stride < vocab || (output && output_stride < vocab))
         return adapt(op, "a row stride is shorter than its row.");
     if (logits_stride > INT32_MAX || output_stride > INT32_MAX) return adapt(op, "a row stride is too large.");
-    const si_logit_controls &c = *controls;
+    si_logit_controls c = *controls;
+    // an empty list is an absent one: the kernel takes a list's starts where its tokens are given, and only those of
+    // a list that is not empty are checked below
+    if (!c.history_count) c.history = c.history_starts = nullptr;
+    if (!c.bias_count) c.bias_tokens = c.bias_starts = nullptr;
     const uint64_t in = span(rows, logits_stride, vocab, size);
     if (si_status st = ports({{"logits", logits, in, size}})) return st;
     if (output) {
@@ -207,7 +211,7 @@ si_status si_process_logits(uint32_t type, const void *logits, int64_t logits_st
         if (si_status st = ports({{"next_token", next_token, per_row, 4}})) return st;
     if (c.history_count < 0 || c.bias_count < 0 || c.history_count > INT32_MAX || c.bias_count > INT32_MAX)
         return adapt(op, "list lengths must be 0 .. 2^31 - 1.");
-    if (c.history && c.history_count)
+    if (c.history)
         if (si_status st = ports({{"history", c.history, uint64_t(c.history_count) * 4, 4},
                                   {"history_starts", c.history_starts, starts, 4}}))
             return st;
@@ -217,7 +221,7 @@ si_status si_process_logits(uint32_t type, const void *logits, int64_t logits_st
         if (si_status st = ports({{"frequency", c.frequency, per_row, 4}})) return st;
     if (c.presence)
         if (si_status st = ports({{"presence", c.presence, per_row, 4}})) return st;
-    if (c.bias_tokens && c.bias_count)
+    if (c.bias_tokens)
         if (si_status st = ports({{"bias_tokens", c.bias_tokens, uint64_t(c.bias_count) * 4, 4},
                                   {"bias_values", c.bias_values, uint64_t(c.bias_count) * 4, 4},
                                   {"bias_starts", c.bias_starts, starts, 4}}))

@@ -164,7 +164,7 @@ __device__ __forceinline__ void walk(const AttentionArgs<T> &g, const Item &it, 
             const int mine = tile + lane, shift = a.page_shift - 4, entry = mine >> shift;
             places = kNone;
             if (mine < t_end && 16 * mine <= any_last && 16 * mine + 15 >= any_first && entry < a.table_width) {
-                const int page = __ldg(a.page_table + int64_t(it.stream) * a.table_width + entry);
+                const int page = a.page_table[int64_t(it.stream) * a.table_width + entry];
                 if (uint32_t(page) < uint32_t(a.page_count))
                     places = ((uint32_t(page) * a.kv_heads + it.kvh) << shift) + (mine & ((1 << shift) - 1));
             }

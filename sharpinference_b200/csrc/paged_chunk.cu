@@ -505,15 +505,17 @@ __global__ void __launch_bounds__(Chunk<T, D>::kThreads, 1) paged_chunk_kernel(c
                 const int mine = low + lane, shift = a.page_shift - 4, entry = mine >> shift;
                 places = kNone;
                 if (16 * mine <= any_last && 16 * mine + 15 >= any_first && entry < a.table_width) {
-                    const int page = __ldg(a.page_table + int64_t(stream) * a.table_width + entry);
+                    const int page = a.page_table[int64_t(stream) * a.table_width + entry];
                     if (uint32_t(page) < uint32_t(a.page_count))
                         places = ((uint32_t(page) * a.kv_heads + kvh) << shift) + (mine & ((1 << shift) - 1));
                 }
             }
             return __shfl_sync(0xffffffffu, places, sub - held);
         };
-        // the loads of step i + 1 travel while step i waits for its place and the products of step i run; one
-        // copy of the code, because the block's four roles share the instruction cache
+        // Pages are read by ordinary loads: this grid may have started beside the append that writes them, and only
+        // those see after pdl_wait() what it wrote (the non-coherent path wants memory that nobody writes while a
+        // grid runs). The loads of step i + 1 travel while step i waits for its place and the products of step i run;
+        // one copy of the code, because the block's four roles share the instruction cache
         auto walk = [&](auto &x, auto &&load, auto &&put) {
             if (steps > 0) load(0, x);
 #pragma unroll 1
@@ -543,12 +545,12 @@ __global__ void __launch_bounds__(Chunk<T, D>::kThreads, 1) paged_chunk_kernel(c
                         const uint4 *w = reinterpret_cast<const uint4 *>(tile + slot * (D / 2));
 #pragma unroll
                         for (int n = 0; n < NG; ++n) {
-                            const uint4 y = __ldg(w + n);
+                            const uint4 y = w[n];
                             x.w[4 * n] = y.x, x.w[4 * n + 1] = y.y, x.w[4 * n + 2] = y.z, x.w[4 * n + 3] = y.w;
                         }
 #pragma unroll
                         for (int n = 0; n < NG / 2; ++n)
-                            x.s[n] = __ldg(reinterpret_cast<const uint32_t *>(tile + 16 * D + slot * (2 * NG)) + n);
+                            x.s[n] = reinterpret_cast<const uint32_t *>(tile + 16 * D + slot * (2 * NG))[n];
                     } else {
 #pragma unroll
                         for (int n = 0; n < NG; ++n) x.w[4 * n] = x.w[4 * n + 1] = x.w[4 * n + 2] = x.w[4 * n + 3] = 0;
@@ -598,8 +600,8 @@ __global__ void __launch_bounds__(Chunk<T, D>::kThreads, 1) paged_chunk_kernel(c
                         const uint32_t *p =
                             reinterpret_cast<const uint32_t *>(tile + 8 * D + 8 * (tg & 1) * (D / 2)) + w;
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) x.w[n][e] = __ldg(p + e * (D / 8));
-                        x.s[n] = __ldg(reinterpret_cast<const uint4 *>(tile + 17 * D + (w >> 2) * 32 + 16 * (tg & 1)));
+                        for (int e = 0; e < 8; ++e) x.w[n][e] = p[e * (D / 8)];
+                        x.s[n] = *reinterpret_cast<const uint4 *>(tile + 17 * D + (w >> 2) * 32 + 16 * (tg & 1));
                     }
                 },
                 [&](int i, RawV<D> &x) {

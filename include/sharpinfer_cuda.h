@@ -190,7 +190,9 @@ si_status si_matrix_multiply_static_workspace(uint32_t weight_type, const float 
  * 1, 2, 4, 8 a full / empty / MMA / epilogue wait ran out; 16 a peer never
  * published its rows; 32 a quantized scale outside the few-row GEMM's FP16
  * operand range (Q8_0 block scale above 512, Q4_K minimum scale above 1024;
- * weights beyond +-65,000), whose rows are then not exact. */
+ * weights beyond +-65,000), whose rows are then not exact; 64 a workspace of
+ * si_paged_attention that was not zeroed before its first call, or that calls
+ * shared at the same time: rows of that call are then left untouched. */
 si_status si_device_error_take(int device, uint32_t *code);
 
 /* ---------------------------------------------------------------------- */

@@ -21,6 +21,7 @@ enum : uint32_t {
     // a Q8_0 block scale above 512 or a Q4_K minimum scale above 1024 reached the
     // few-row GEMM's FP16 operands (gemm_fewrow.cu): those rows are not exact
     kErrRange = 32u,
+    kErrNoSlot = 64u,  // a workspace's slots were all taken: not zeroed, or shared by calls that overlap
 };
 static __device__ uint32_t g_error_word;
 

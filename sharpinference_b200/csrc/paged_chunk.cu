@@ -359,14 +359,18 @@ __global__ void __launch_bounds__(Chunk<T, D>::kThreads, 1) paged_chunk_kernel(c
             // registers allow one block an SM, so its SM's is free; were it not, another is
             uint32_t sm;
             asm volatile("mov.u32 %0, %%smid;" : "=r"(sm));
-            for (int k = 0; k < g.slots; ++k) {
-                slot_of = int((sm + k) % uint32_t(g.slots));
-                if (atomicCAS(g.tickets + slot_of, 0u, 1u) == 0u) break;
+            slot_of = -1;
+            for (int k = 0; k < g.slots && slot_of < 0; ++k) {
+                const int slot = int((sm + k) % uint32_t(g.slots));
+                if (atomicCAS(g.tickets + slot, 0u, 1u) == 0u) slot_of = slot;
             }
+            // none: the workspace was not zeroed, or another call uses it at the same time
+            if (slot_of < 0) atomicOr(&g_error_word, kErrNoSlot);
         }
     }
     __syncthreads();
     const int stream = found[0], pass = found[1];
+    if (borrow && slot_of < 0) return;
     Place at;
     if (stream >= 0) at = place_at(a, g.group, g.window, kBlockRows, splits, stream, pass, kvh, part);
     if (stream < 0 || (kCut && part >= at.parts)) {

@@ -62,3 +62,32 @@ def test_chunks_read_what_the_append_before_them_wrote(torch, type, rows, past, 
             err = np.abs(out[i].double().cpu().numpy() - want)
             assert (err <= ref.attention_bound(s, weight, reach, want, type == N.F16)).all()
         s.lengths = final
+
+
+def test_a_workspace_without_a_free_slot_is_reported(torch):
+    """Sums of many blocks of an F32 chunk lie in slots that the blocks take turns with. A workspace that was not
+    zeroed has none to give: the call says so and writes nothing."""
+    d, heads, rows = 64, 1, 3000
+    s = ref.Streams(np.random.default_rng(7), [rows] * 16, 1, d, 256)
+    dev = Device(torch, s)
+    starts, lengths = dev.rows([rows] * 16)
+    q = torch.randn(rows * 16, d, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    ws = torch.full((native.paged_attention_workspace_bytes(dev.cache, rows * 16, rows, heads),), 1, dtype=torch.uint8,
+                    device="cuda")
+    out = torch.full_like(q, 7.0)
+
+    def attend():
+        torch.cuda.synchronize()
+        native.call("si_paged_attention", C.byref(dev.cache), N.F32, q.data_ptr(), d, starts.data_ptr(),
+                    lengths.data_ptr(), out.data_ptr(), d, rows * 16, rows, heads, 0.125, 0, ws.data_ptr(), ws.numel(),
+                    None)
+        torch.cuda.synchronize()
+
+    attend()
+    assert native.device_error_take(0) == 64
+    assert (out == 7.0).all()
+    ws.zero_()
+    attend()
+    assert native.device_error_take(0) == 0
+    v = torch.from_numpy(np.stack([x[0, 0] for x in s.values])).cuda()  # first rows see their own token alone
+    assert torch.allclose(out.view(16, rows, d)[:, 0].double(), v, rtol=1e-5, atol=0)

@@ -489,8 +489,8 @@ si_status si_paged_kv_gather(const si_paged_cache *cache, uint32_t type, const i
  * holds; out = softmax(scale * q . k) v with query head h on key/value head
  * h / (query_heads / kv_heads). A row that sees no token gets zeros. Serves
  * single tokens, a few drafted rows and prompt chunks, mixed in one call;
- * max_rows bounds the rows of one stream (1 for a decode step) and picks the
- * kernel. The keys and values of the rows themselves must have been appended.
+ * max_rows, the most rows of one stream (1 for a decode step), picks the
+ * kernel; a stream with more rows gets the same answers. The keys and values of the rows themselves must have been appended.
  * `workspace`: device scratch of si_paged_attention_workspace_bytes(...),
  * 16-byte aligned, zeroed once before its first call; each call leaves it ready for the
  * next one, and calls that share it must be ordered on one stream. */

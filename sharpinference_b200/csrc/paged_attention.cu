@@ -44,6 +44,10 @@ using namespace si::dev;
 // 74/72 and 100/73; one of 32768, F32 64 pairs 57/72, 96 pairs 79/74, F16 44 pairs 41/55, 96 pairs 71/56.
 constexpr int kFewPairs = 32;
 constexpr int kPairs = 8;         // pairs of a row and a head in one pass
+template <bool kFour>
+constexpr int pass_pairs() {  // where rows or columns of the products hold a pair twice (`walk`)
+    return kFour ? kPairs / 2 : kPairs;
+}
 
 // N words from shared memory by the widest loads that N allows.
 template <int N>
@@ -120,7 +124,7 @@ struct Sums {
     uint32_t bad;  // groups in which the lane's pair sees a value that is not finite
 };
 
-// An item: one pass of eight pairs of one stream on one key/value head.
+// An item: one pass of eight (four) pairs of one stream on one key/value head.
 struct Item {
     StreamWork sw;
     int stream, kvh, pass;
@@ -128,7 +132,7 @@ struct Item {
 };
 
 // One warp over the tiles [tile_a, tile_b) of an item, two at a time through its
-// ring of two stages. kFour (32-bit calls of up to four pairs a stream): rows lg and
+// ring of two stages. kFour (32-bit calls of up to four pairs a stream, passes of four): rows lg and
 // lg + 4 of the scores are the same pair, and the probabilities' columns lg + 4
 // hold what rounding left of columns lg, so that one product does for both (64
 // streams of 4 pairs: 86.2 us against 90.0).
@@ -141,7 +145,7 @@ __device__ __forceinline__ void walk(const AttentionArgs<T> &g, const Item &it, 
     const StreamWork &sw = it.sw;
     const int lane = threadIdx.x & 31, lg = lane >> 2, lt = lane & 3;
     // this lane's pair: the queries as A fragments and its visible tokens
-    const int pair = it.pass * kPairs + (kFour ? lg & 3 : lg), row_in = pair / g.group;
+    const int pair = it.pass * pass_pairs<kFour>() + (kFour ? lg & 3 : lg), row_in = pair / g.group;
     const bool live = row_in < sw.rows;
     const T *src = g.query + (sw.begin + row_in) * g.query_stride + int64_t(it.kvh * g.group + pair - row_in * g.group) * D;
     const int position = live ? sw.length - sw.rows + row_in : -1;
@@ -490,10 +494,10 @@ __device__ __forceinline__ void deposit(const Sums<D> &r, float *slot) {
 }
 
 // Output row and head of a pair of an item; null for a pair without an output.
-template <class T, int D>
+template <class T, int D, bool kFour>
 __device__ __forceinline__ T *pair_output(const AttentionArgs<T> &g, const Item &it, int pr) {
-    const int pair = it.pass * kPairs + pr, row = pair / g.group;
-    if (row >= it.sw.rows) return nullptr;
+    const int pair = it.pass * pass_pairs<kFour>() + pr, row = pair / g.group;
+    if (pr >= pass_pairs<kFour>() || row >= it.sw.rows) return nullptr;
     const int p = it.sw.length - it.sw.rows + row;
     if (p < 0 || (p >> g.a.page_shift) >= g.a.table_width) return nullptr;
     return g.output + (it.sw.begin + row) * g.output_stride + int64_t(it.kvh * g.group + pair - row * g.group) * D;
@@ -506,19 +510,20 @@ struct Parts {
     __device__ __forceinline__ const float *at(int i) const { return i == 0 ? first : rest + int64_t(i) * stride; }
 };
 
+template <bool kFour>
 __device__ __forceinline__ int live_pairs(const Item &it, int group) {
-    return min(kPairs, it.sw.rows * group - it.pass * kPairs);
+    return min(pass_pairs<kFour>(), it.sw.rows * group - it.pass * pass_pairs<kFour>());
 }
 
 // Adds the parts of an item up, in their order: the pairs who, who + many, .. by
 // this warp, written as output (`part` null) or as one part of the whole. A lane
 // holds a part's factor; there are no more parts than warps in a block.
-template <class T, int D>
+template <class T, int D, bool kFour>
 __device__ __forceinline__ void combine(const AttentionArgs<T> &g, const Item &it, const Parts &ps, int who, int many,
                                         float *part) {
     constexpr int V = D % 128 ? 2 : 4, C = D / 32 / V;  // a lane's channels: C vectors of V
     using Vec = typename std::conditional<V == 4, float4, float2>::type;
-    const int lane = threadIdx.x & 31, live = live_pairs(it, g.group);
+    const int lane = threadIdx.x & 31, live = live_pairs<kFour>(it, g.group);
 #pragma unroll 1
     for (int pr = who; pr < live; pr += many) {
         float m = -INFINITY, l = 0.0f;
@@ -563,7 +568,7 @@ __device__ __forceinline__ void combine(const AttentionArgs<T> &g, const Item &i
                 __stcg(part + kPairs * D + pr, top);
                 __stcg(part + kPairs * D + kPairs + pr, sum);
             }
-        } else if (T *out = pair_output<T, D>(g, it, pr)) {
+        } else if (T *out = pair_output<T, D, kFour>(g, it, pr)) {
             const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll
             for (int c = 0; c < C; ++c)
@@ -578,16 +583,16 @@ __device__ __forceinline__ void combine(const AttentionArgs<T> &g, const Item &i
 // with them: what this costs is its loads' latency (one stream of 32768 tokens: 28 us so, 35 us with a pass over the
 // maxima first and four loads at a time). Both joins are inlined: handed over in
 // local memory, their arguments cost the 64 streams 10 us of 86.
-template <class T, int D, int NW>
+template <class T, int D, bool kFour, int NW>
 __device__ __forceinline__ void combine_blocks(const AttentionArgs<T> &g, const Item &it, const Parts &ps, int warp) {
     constexpr int CH = D / 32;  // a lane's channels
     constexpr int V = CH % 4 == 0 ? 4 : CH % 2 == 0 ? 2 : 1, RUN = CH <= 2 ? 16 : 8;
     using Vec = typename std::conditional<V == 4, float4, typename std::conditional<V == 2, float2, float>::type>::type;
     const int lane = threadIdx.x & 31;
 #pragma unroll 1
-    for (int pr = warp; pr < kPairs; pr += NW) {
+    for (int pr = warp; pr < pass_pairs<kFour>(); pr += NW) {
         const int from = pr * D;
-        T *out = pair_output<T, D>(g, it, pr);
+        T *out = pair_output<T, D, kFour>(g, it, pr);
         if (!out) continue;
         float acc[CH], top = -INFINITY, sum = 0.0f;
 #pragma unroll
@@ -635,7 +640,7 @@ __device__ __forceinline__ void combine_blocks(const AttentionArgs<T> &g, const 
     }
 }
 
-template <class T, int D>
+template <class T, int D, bool kFour>
 __device__ __forceinline__ void finish(const AttentionArgs<T> &g, const Item &it, const Sums<D> &r) {
     constexpr int W = D / 64;
     const int lane = threadIdx.x & 31, lg = lane >> 2, lt = lane & 3;
@@ -643,7 +648,7 @@ __device__ __forceinline__ void finish(const AttentionArgs<T> &g, const Item &it
     for (int c = 0; c < 2; ++c) {
         const uint32_t bad = __shfl_sync(0xffffffffu, r.bad, 8 * lt + 4 * c);
         const float l = __shfl_sync(0xffffffffu, r.l, 8 * lt + 4 * c);
-        T *out = pair_output<T, D>(g, it, 2 * lt + c);
+        T *out = pair_output<T, D, kFour>(g, it, 2 * lt + c);
         const float inv = l != 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
@@ -683,7 +688,7 @@ __device__ __forceinline__ int inclusive(int v) {
 
 // Every warp finds its cut by itself: a lane adds up a run of streams, the lane
 // whose run the cut begins in is found, then the stream in the run.
-template <int NW>
+template <int NW, int kPass>
 __device__ __forceinline__ bool find_cut(const PagedArgs &a, int group, int window, int min_share, Cut &c) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = (a.streams + 31) / 32;
     const int b0 = min(lane * per, a.streams), b1 = min(b0 + per, a.streams);
@@ -691,7 +696,7 @@ __device__ __forceinline__ bool find_cut(const PagedArgs &a, int group, int wind
     int mine = 0;
     StreamWork w;
     for (int b = b0; b < b1; ++b) {
-        w = stream_work(a, b, group, window, kPairs);
+        w = stream_work(a, b, group, window, kPass);
         mine += line_tiles(a, w, c);
     }
     const int total = __reduce_add_sync(0xffffffffu, mine), warps_all = int(gridDim.x) * NW;
@@ -700,7 +705,7 @@ __device__ __forceinline__ bool find_cut(const PagedArgs &a, int group, int wind
     c.block = NW * c.share;
     int blocks = 0;  // at most the tiles, so no overflow
     for (int b = b0; b < b1; ++b) {
-        if (per > 1) w = stream_work(a, b, group, window, kPairs);
+        if (per > 1) w = stream_work(a, b, group, window, kPass);
         blocks += w.passes * a.kv_heads * ((w.tiles + c.block - 1) / c.block);
     }
     c.padded = __reduce_add_sync(0xffffffffu, blocks) <= int(gridDim.x);
@@ -716,7 +721,7 @@ __device__ __forceinline__ bool find_cut(const PagedArgs &a, int group, int wind
     c.stream = k * per;
     while (per > 1) {
         const int b = c.stream + lane;
-        w = stream_work(a, min(b, a.streams - 1), group, window, kPairs);
+        w = stream_work(a, min(b, a.streams - 1), group, window, kPass);
         const int tiles = b < a.streams ? line_tiles(a, w, c) : 0;
         const int upto = c.stream_at + inclusive(tiles);
         const uint32_t past = __ballot_sync(0xffffffffu, upto > c.begin);
@@ -748,7 +753,7 @@ __global__ void __launch_bounds__(warps<D>() * 32, 1) paged_attention_kernel(con
     const PagedArgs &a = g.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     Cut cut;
-    if (!find_cut<NW>(a, g.group, g.window, g.min_share, cut)) return;
+    if (!find_cut<NW, pass_pairs<kFour>()>(a, g.group, g.window, g.min_share, cut)) return;
     if (threadIdx.x < 2) merge_first[threadIdx.x] = -1;
 
     float *tail_slot = smem + warp * WF, *head_slot = tail_slot + RF;
@@ -763,7 +768,7 @@ __global__ void __launch_bounds__(warps<D>() * 32, 1) paged_attention_kernel(con
             const int span = cut.padded ? (it.sw.tiles + cut.block - 1) / cut.block * cut.block : it.sw.tiles;
             if (x >= cut.stream_at + span * items) {
                 cut.stream_at += span * items;
-                it.sw = stream_work(a, ++it.stream, g.group, g.window, kPairs);
+                it.sw = stream_work(a, ++it.stream, g.group, g.window, pass_pairs<kFour>());
                 continue;
             }
             const int index = (x - cut.stream_at) / span;
@@ -784,7 +789,7 @@ __global__ void __launch_bounds__(warps<D>() * 32, 1) paged_attention_kernel(con
                 __syncwarp();
                 deposit<D>(r, has_tail ? tail_slot : head_slot);
             } else {
-                finish<T, D>(g, it, r);
+                finish<T, D, kFour>(g, it, r);
             }
             x = stop;
         }
@@ -807,7 +812,7 @@ __global__ void __launch_bounds__(warps<D>() * 32, 1) paged_attention_kernel(con
         ps.stride = WF;
         ps.n = (min(end, block_end) - block_begin + cut.share - 1) / cut.share - lead;
         // slot 0 of a block: an item that began in an earlier one, slot 1: in it
-        combine<T, D>(g, c, ps, warp - lead, ps.n,
+        combine<T, D, kFour>(g, c, ps, warp - lead, ps.n,
                       whole ? nullptr : g.parts + (2 * int64_t(blockIdx.x) + here) * PF);
         if (!whole) {
             divided = true;
@@ -836,7 +841,7 @@ __global__ void __launch_bounds__(warps<D>() * 32, 1) paged_attention_kernel(con
         ps.rest = ps.first - PF;
         ps.stride = 2 * PF;
         ps.n = merge_last[slot] - merge_first[slot] + 1;
-        combine_blocks<T, D, NW>(g, merge_item[slot], ps, warp);
+        combine_blocks<T, D, kFour, NW>(g, merge_item[slot], ps, warp);
     }
 }
 
@@ -846,7 +851,8 @@ template <class T, int D, bool kFour>
 si_status launch(const AttentionArgs<T> &g, void *stream) {
     constexpr int NW = warps<D>();
     const double tiles = double(int64_t(g.a.table_width) << (g.a.page_shift - 4));
-    const double passes = double((g.a.rows * g.group + kPairs - 1) / kPairs + g.a.streams);
+    constexpr int kPass = pass_pairs<kFour>();
+    const double passes = double((g.a.rows * g.group + kPass - 1) / kPass + g.a.streams);
     const double most = tiles * passes * g.a.kv_heads;
     if (most > double(INT32_MAX / 2))
         return fail(SI_ERR_UNSUPPORTED, "paged-attention: rows times the table's tokens exceed 2^30 tiles.");
@@ -879,7 +885,7 @@ si_status run(const PagedArgs &a, const PagedAttention &q, void *stream) {
                              reinterpret_cast<float *>(static_cast<uint8_t *>(q.workspace) + ticket_bytes()),
                              device_sm_count(), 1};
     if (int64_t(q.max_rows) * g.group > kFewPairs) return paged_chunk_attention(g, stream);
-    if (sizeof(T) == 4 && int64_t(q.max_rows) * g.group <= kPairs / 2) return launch_size<T, sizeof(T) == 4>(g, stream);
+    if (sizeof(T) == 4 && int64_t(q.max_rows) * g.group <= pass_pairs<true>()) return launch_size<T, sizeof(T) == 4>(g, stream);
     return launch_size<T, false>(g, stream);
 }
 

@@ -468,7 +468,8 @@ si_status si_paged_cache_bytes(int64_t page_count, int32_t page_size, int32_t kv
  * token at position lengths[b] - (row_starts[b + 1] - r). Both are read on the
  * device: one recorded graph serves every step. Rows of no stream, and rows
  * whose position is outside [0, table_width * page_size), are left untouched.
- * Tensors are F32 or F16 (`type`); strides count elements.
+ * Tensors are F32 or F16 (`type`); strides count elements. What a call writes
+ * may not overlap what it reads.
  *
  * transformer.rope-kv-write into pages: row = [query | key | value] heads;
  * query and key heads are rotated as si_rope_kv_write rotates them

@@ -29,6 +29,14 @@ si_status ports(std::initializer_list<Port> list) {
     return SI_OK;
 }
 
+// What a call writes may not lie in what its other blocks still read.
+si_status apart(const Port &written, std::initializer_list<Port> read) {
+    for (const Port &p : read)
+        if (p.ptr && p.bytes && ranges_overlap(written.ptr, written.bytes, p.ptr, p.bytes))
+            return fail(SI_ERR_INVALID_ARGUMENT, "port '%s': overlaps port '%s'", written.name, p.name);
+    return SI_OK;
+}
+
 si_status tensor_type(const char *op, uint32_t type, uint32_t *size) {
     if (type != SI_TYPE_F32 && type != SI_TYPE_F16)
         return fail(SI_ERR_ADAPTATION, "%s: tensors must be F32 or F16.", op);
@@ -78,6 +86,15 @@ si_status cache_ports(const si_paged_cache *c, const PagedArgs &a) {
                   {"lengths", a.lengths, uint64_t(a.streams) * 4, 4}});
 }
 
+// A written tensor against the cache and the row descriptors.
+si_status apart_from_cache(const Port &written, const si_paged_cache *c, const PagedArgs &a) {
+    return apart(written,
+                 {{"pages", a.pages, page_bytes(c->page_size, a.kv_heads, a.head_size) * uint64_t(a.page_count), 16},
+                  {"page_table", a.page_table, uint64_t(a.streams) * uint64_t(a.table_width) * 4, 4},
+                  {"row_starts", a.row_starts, uint64_t(a.streams + 1) * 4, 4},
+                  {"lengths", a.lengths, uint64_t(a.streams) * 4, 4}});
+}
+
 si_status attention_shape(const char *op, const PagedArgs &a, int32_t max_rows, int32_t query_heads) {
     if (query_heads <= 0 || max_rows <= 0) return adapt(op, "dimensions must be positive.");
     if (query_heads % a.kv_heads) return adapt(op, "Query heads must be divisible by key/value heads.");
@@ -116,6 +133,12 @@ si_status si_paged_rope_kv_append(const si_paged_cache *cache, uint32_t type, co
     if (qkv_stride > INT32_MAX || query_stride > INT32_MAX) return adapt(op, "a row stride is too large.");
     const uint64_t in = span(rows, qkv_stride, width, size), out = span(rows, query_stride, q, size);
     if (ranges_overlap(query, out, qkv, in)) return fail(SI_ERR_UNSUPPORTED, "%s: output aliases an input.", op);
+    if (si_status st = apart_from_cache({"query", query, out, size}, cache, a)) return st;
+    if (si_status st = apart({"query", query, out, size}, {{"frequencies", frequencies, uint64_t(rotary_size / 2) * 4, 4}}))
+        return st;
+    if (si_status st = apart({"pages", a.pages, page_bytes(cache->page_size, a.kv_heads, a.head_size) * uint64_t(a.page_count), 16},
+                             {{"qkv", qkv, in, size}}))
+        return st;
     if (si_status st = cache_ports(cache, a)) return st;
     if (si_status st = ports({{"qkv", qkv, in, size}, {"query", query, out, size}})) return st;
     if (rotary_size)
@@ -133,6 +156,8 @@ si_status si_paged_kv_gather(const si_paged_cache *cache, uint32_t type, const i
     if (si_status st = cache_args(op, cache, row_starts, lengths, rows, &a)) return st;
     const uint64_t bytes = uint64_t(rows) * a.kv_heads * a.head_size * size;
     if (ranges_overlap(keys, bytes, values, bytes)) return fail(SI_ERR_UNSUPPORTED, "%s: outputs overlap.", op);
+    if (si_status st = apart_from_cache({"keys", keys, bytes, size}, cache, a)) return st;
+    if (si_status st = apart_from_cache({"values", values, bytes, size}, cache, a)) return st;
     if (si_status st = cache_ports(cache, a)) return st;
     if (si_status st = ports({{"keys", keys, bytes, size}, {"values", values, bytes, size}})) return st;
     return kernels::paged_gather(a, type, keys, values, stream);
@@ -171,6 +196,9 @@ si_status si_paged_attention(const si_paged_cache *cache, uint32_t type, const v
     const uint64_t in = span(rows, query_stride, width, size), out = span(rows, output_stride, width, size);
     if (ranges_overlap(output, out, query, in) || (need && ranges_overlap(output, out, workspace, need)))
         return fail(SI_ERR_UNSUPPORTED, "%s: output aliases an input.", op);
+    if (si_status st = apart_from_cache({"output", output, out, size}, cache, a)) return st;
+    if (si_status st = apart_from_cache({"workspace", workspace, need, 16}, cache, a)) return st;
+    if (si_status st = apart({"workspace", workspace, need, 16}, {{"query", query, in, size}})) return st;
     if (si_status st = cache_ports(cache, a)) return st;
     if (si_status st = ports({{"query", query, in, size}, {"output", output, out, size}})) return st;
     if (need)

@@ -70,11 +70,15 @@ si_status cache_args(const char *op, const si_paged_cache *c, const int32_t *row
     if (c->streams <= 0 || c->table_width <= 0 || rows <= 0) return adapt(op, "dimensions must be positive.");
     if (int64_t(c->table_width) * c->page_size > INT32_MAX || rows > INT32_MAX)
         return adapt(op, "more than 2^31 - 1 tokens.");
-    if (!row_starts && rows != c->streams) return adapt(op, "without row_starts there is one row per stream.");
     int shift = 4;
     while ((16 << (shift - 4)) < c->page_size) ++shift;
     *out = PagedArgs{static_cast<uint8_t *>(c->pages), c->page_table, row_starts, lengths, c->page_count, rows,
                      c->streams, c->table_width, shift, c->kv_heads, c->head_size};
+    return SI_OK;
+}
+
+si_status rows_of_streams(const char *op, const PagedArgs &a) {
+    if (!a.row_starts && a.rows != a.streams) return adapt(op, "without row_starts there is one row per stream.");
     return SI_OK;
 }
 
@@ -123,6 +127,7 @@ si_status si_paged_rope_kv_append(const si_paged_cache *cache, uint32_t type, co
     PagedArgs a;
     if (si_status st = tensor_type(op, type, &size)) return st;
     if (si_status st = cache_args(op, cache, row_starts, lengths, rows, &a)) return st;
+    if (si_status st = rows_of_streams(op, a)) return st;
     if (si_status st = attention_shape(op, a, 1, query_heads)) return st;
     if (rotary_size < 0 || rotary_size > a.head_size || rotary_size % 2)
         return adapt(op, "Invalid query, cache, head, or rotary dimensions.");
@@ -154,6 +159,7 @@ si_status si_paged_kv_gather(const si_paged_cache *cache, uint32_t type, const i
     PagedArgs a;
     if (si_status st = tensor_type(op, type, &size)) return st;
     if (si_status st = cache_args(op, cache, row_starts, lengths, rows, &a)) return st;
+    if (si_status st = rows_of_streams(op, a)) return st;
     const uint64_t bytes = uint64_t(rows) * a.kv_heads * a.head_size * size;
     if (ranges_overlap(keys, bytes, values, bytes)) return fail(SI_ERR_UNSUPPORTED, "%s: outputs overlap.", op);
     if (si_status st = apart_from_cache({"keys", keys, bytes, size}, cache, a)) return st;
@@ -168,7 +174,7 @@ si_status si_paged_attention_workspace_bytes(const si_paged_cache *cache, int64_
     const char *op = "paged-attention";
     if (!bytes) return fail(SI_ERR_INVALID_ARGUMENT, "null argument");
     PagedArgs a;
-    if (si_status st = cache_args(op, cache, cache ? cache->page_table : nullptr, nullptr, rows, &a)) return st;
+    if (si_status st = cache_args(op, cache, nullptr, nullptr, rows, &a)) return st;
     if (si_status st = attention_shape(op, a, max_rows, query_heads)) return st;
     *bytes = kernels::paged_attention_workspace(a, rows, max_rows, query_heads);
     return SI_OK;
@@ -183,6 +189,7 @@ si_status si_paged_attention(const si_paged_cache *cache, uint32_t type, const v
     PagedArgs a;
     if (si_status st = tensor_type(op, type, &size)) return st;
     if (si_status st = cache_args(op, cache, row_starts, lengths, rows, &a)) return st;
+    if (si_status st = rows_of_streams(op, a)) return st;
     if (si_status st = attention_shape(op, a, max_rows, query_heads)) return st;
     if (!std::isfinite(scale) || scale <= 0.0f) return adapt(op, "Attribute 'scale' must be finite and positive.");
     if (window < 0) return adapt(op, "Attribute 'window' must be non-negative.");

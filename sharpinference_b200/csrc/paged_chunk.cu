@@ -700,9 +700,10 @@ __global__ void __launch_bounds__(Chunk<T, D>::kThreads, 1) paged_chunk_kernel(c
         };
         const int phase = flush_phase(own);
         bool begun = false;    // the slot holds something
-        int emptied = 0;       // the step that began the present sums
-        // what the mean of their truncations makes good, for a product of four for either half in each step
-        auto untruncated = [&](int i) { return kWide ? 1.0f + 4.0f * kTruncated * float(i - emptied) : 1.0f; };
+        int summed = 0;        // products of 16 tokens that put something into the present sums of the row
+        // what the mean of their truncations makes good: one product adds either half; where the row sees none of the
+        // 16 tokens it adds zeros, which lose nothing
+        auto untruncated = [&] { return kWide ? 1.0f + kTruncated * float(summed) : 1.0f; };
         float flushed = 1.0f;  // how far the maximum has moved since the slot was written
         float m = -INFINITY, l = 0.0f, most = -INFINITY;
         bool ok = true;
@@ -723,9 +724,9 @@ __global__ void __launch_bounds__(Chunk<T, D>::kThreads, 1) paged_chunk_kernel(c
                     break;
                 }
                 tc_fence_after();
-                flush(begun, flushed, untruncated(i));
+                flush(begun, flushed, untruncated());
                 begun = true;
-                emptied = i;
+                summed = 0;
                 flushed = 1.0f;
             }
             const uint32_t have = mapped[i & 7];
@@ -741,9 +742,12 @@ __global__ void __launch_bounds__(Chunk<T, D>::kThreads, 1) paged_chunk_kernel(c
                     if (lo > 0 && lo < 32) sees &= 0xffffffffu << lo;
                     if (!((have >> (c / 2)) & 1u)) sees &= 0xffff0000u;
                     if (!((have >> (c / 2 + 8)) & 1u)) sees &= 0x0000ffffu;
+                    if constexpr (kWide) summed += int((sees & 0xffffu) != 0) + int((sees >> 16) != 0);
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[c + j] = (sees >> j) & 1u ? v[c + j] : 0xff800000u;
                 }
+            } else if constexpr (kWide) {
+                summed += kTokens / 16;
             }
             float top = -INFINITY, other = -INFINITY;
 #pragma unroll
@@ -833,7 +837,7 @@ __global__ void __launch_bounds__(Chunk<T, D>::kThreads, 1) paged_chunk_kernel(c
         }
         if (kCut && ok && at.parts > 1) {  // one part of the row's sums, for the join
             if (my_steps > 0) {
-                flush(begun, flushed, untruncated(steps));
+                flush(begun, flushed, untruncated());
                 float *stats = g.parts + int64_t(slot_of) * C::kSlot + kBlockRows * D + tid;
                 __stcg(stats, m * unscale);
                 __stcg(stats + kBlockRows, l);
@@ -842,7 +846,7 @@ __global__ void __launch_bounds__(Chunk<T, D>::kThreads, 1) paged_chunk_kernel(c
             }
         } else if (ok) {
             const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-            const float whole = untruncated(steps);
+            const float whole = untruncated();
             float4 held[8];  // what the slot holds of the next 32 channels
             auto fetch = [&](int c) {
 #pragma unroll

@@ -15,19 +15,19 @@
 //     them to F16 left over.
 // The tiles of 16 tokens of all streams, heads and passes form one line that is
 // cut evenly over the warps of the grid, so uneven lengths balance. A warp walks
-// its cut with running maxima that move only when a score exceeds them by 2^7,
+// its cut with running maxima that move only when a score exceeds them by 2^2,
 // the next two tiles on their way into its ring; items that a cut divides are put together
 // in shared memory once per block, and over the blocks by the last to arrive.
 // Measured: 64 streams of up to 4096 tokens (40 query, 10 key/value heads of 128,
 // F32) 72 us, 3.2 TB/s: near half each of the ALU, FMA and tensor pipes at the
 // three warps a scheduler that the registers allow. One stream of 32768 tokens (24, 8
 // heads) 22.6 us, of which the tiles take 11.5.
-// F16 probabilities end 2^-32 below a row's largest. In an F32 row that
+// F16 probabilities end 2^-37 below a row's largest. In an F32 row that
 // one token owns (all others together below 2^-16 of it) the channels in which
 // that token's value is 0 consist of such small ones, so a warp that meets
 // such a row goes over its tiles once more for it alone, in FP32. Where several
 // tokens own a row and all are 0 in a channel, the rest keeps that floor: it is
-// off by 2^-33 of the largest probability times a value.
+// off by 2^-38 of the largest probability times a value (2^-33 where maxima may lag 2^7, at the same speed).
 #include <type_traits>
 
 #include "launch.cuh"
@@ -43,6 +43,8 @@ using namespace si::dev;
 // 78/67, F16 24 pairs 30/36, 32 pairs 35/35, 44 pairs 46/36; 64 of 1500, F32 32 pairs 81/101, 44 pairs 110/102, F16
 // 74/72 and 100/73; one of 32768, F32 64 pairs 57/72, 96 pairs 79/74, F16 44 pairs 41/55, 96 pairs 71/56.
 constexpr int kFewPairs = 32;
+constexpr float kSlack = 2.0f;    // log2 of what a score may exceed the running maximum by
+constexpr float kLift = 13.0f;    // log2 of a probability at the maximum: F16 keeps more small ones
 constexpr int kPairs = 8;         // pairs of a row and a head in one pass
 template <bool kFour>
 constexpr int pass_pairs() {  // where rows or columns of the products hold a pair twice (`walk`)

@@ -7,8 +7,6 @@
 
 namespace si::dev {
 
-constexpr float kSlack = 7.0f;    // log2 of what a score may exceed the running maximum by (2 makes chunks 8 to 11 % slower)
-constexpr float kLift = 8.0f;     // log2 of a probability at the maximum: F16 keeps more small ones
 constexpr float kOwned = 0x1p-16f; // share of all other tokens in a row that one token owns
 
 template <class T>

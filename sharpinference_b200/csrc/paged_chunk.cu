@@ -46,6 +46,8 @@ constexpr int kTokens = 64;  // of one step: N of the scores, K of the values
 // little where signs are mixed, but as much again where all products of 1024 tokens have one (2.5e-6 of their sum
 // stays lost; a factor that put that back too would be 2.4e-6 too large for mixed signs).
 constexpr float kTruncated = 0.72134752f * 0x1p-24f;
+constexpr float kSlack = 7.0f;  // log2 of what a score may exceed the running maximum by (2 makes chunks 8 to 11 % slower)
+constexpr float kLift = 8.0f;   // log2 of a probability at the maximum: F16 keeps more small ones
 constexpr int kMostParts = 32;
 constexpr int kUnpackK = 64, kUnpackV = 128;  // threads: with the rest 16 warps, which leaves 128 registers to each
 

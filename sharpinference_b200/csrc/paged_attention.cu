@@ -25,13 +25,13 @@
 // F16 probabilities end 2^-37 below a row's largest. In an F32 row that
 // one token owns (all others together below 2^-16 of it) the channels in which
 // that token's value is 0 consist of such small ones, so a warp that meets
-// such a row goes over its tiles once more for it alone, in FP32. Where several
+// such rows goes over its tiles again for them (`sum_windows`). Where several
 // tokens own a row and all are 0 in a channel, the rest keeps that floor: it is
 // off by 2^-38 of the largest probability times a value (2^-33 where maxima may lag 2^7, at the same speed).
 #include <type_traits>
 
 #include "launch.cuh"
-#include "paged_attention.cuh"
+#include "paged_fragments.cuh"
 
 namespace si::kernels {
 namespace {
@@ -45,67 +45,9 @@ using namespace si::dev;
 constexpr int kFewPairs = 32;
 constexpr float kSlack = 2.0f;    // log2 of what a score may exceed the running maximum by
 constexpr float kLift = 13.0f;    // log2 of a probability at the maximum: F16 keeps more small ones
-constexpr int kPairs = 8;         // pairs of a row and a head in one pass
 template <bool kFour>
 constexpr int pass_pairs() {  // where rows or columns of the products hold a pair twice (`walk`)
     return kFour ? kPairs / 2 : kPairs;
-}
-
-// N words from shared memory by the widest loads that N allows.
-template <int N>
-__device__ __forceinline__ void load_words(uint32_t (&dst)[N], const uint8_t *p) {
-    if constexpr (N % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < N; i += 4) {
-            const uint4 x = reinterpret_cast<const uint4 *>(p)[i / 4];
-            dst[i] = x.x, dst[i + 1] = x.y, dst[i + 2] = x.z, dst[i + 3] = x.w;
-        }
-    } else if constexpr (N % 2 == 0) {
-#pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            const uint2 x = reinterpret_cast<const uint2 *>(p)[i / 2];
-            dst[i] = x.x, dst[i + 1] = x.y;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) dst[i] = reinterpret_cast<const uint32_t *>(p)[i];
-    }
-}
-
-// A warp copies one tile into its ring. Four lanes t of a fragment read value
-// rows 4 t + i together, a multiple of 128 B apart: their 16-byte chunks are
-// exchanged (chunk ^ 2 t) so that they lie in different banks.
-template <int D>
-__device__ __forceinline__ void copy_tile(uint8_t *dst, const uint8_t *src) {
-    constexpr int kChunks = tile_bytes(D) / 16, kValues = D / 2;
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int i = 0; i < (kChunks + 31) / 32; ++i) {
-        const int c = lane + 32 * i;
-        int to = c;
-        if (32 * i + 31 >= kValues && 32 * i < 2 * kValues)
-            if (c >= kValues && c < 2 * kValues) to = c ^ ((((c - kValues) / (D / 8)) & 3) << 1);
-        if (32 * i + 31 < kChunks || c < kChunks)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst + 16 * to)), "l"(src + 16 * c)
-                         : "memory");
-    }
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 // Warps of a block, one block to an SM: as many as registers and rings allow, equally many for each of the four
@@ -132,6 +74,34 @@ struct Item {
     int stream, kvh, pass;
     int at, tiles;  // its place on the line
 };
+
+// Sums of those pairs of an item anew that one token owns (the maxima before their scale).
+template <class T, int D, bool kFour>
+__device__ __noinline__ void look_again(const AttentionArgs<T> &g, const Item &it, int tile_a, int tile_b, bool owned, uint8_t *ring,
+                                        Sums<D> &r) {
+    constexpr int W = D / 64;
+    const int lane = threadIdx.x & 31, lg = lane >> 2, lt = lane & 3;
+    const int pair = it.pass * pass_pairs<kFour>() + lg, row = pair / g.group;
+    OwnedPair<T> p;
+    p.live = owned;
+    p.query = g.query + (it.sw.begin + row) * g.query_stride + int64_t(it.kvh * g.group + pair - row * g.group) * D;
+    p.position = it.sw.length - it.sw.rows + row;
+    p.first = g.window ? max(0, p.position - g.window + 1) : 0;
+    const int t_begin = it.sw.first_tile + tile_a, t_end = it.sw.first_tile + tile_b;
+    float us, *part = reinterpret_cast<float *>(ring);
+    const Windows w = find_windows<T, D>(g.a, g.scale, p, it.stream, it.kvh, t_begin, t_end, ring, &us);
+    sum_windows<T, D>(g.a, g.scale, p, it.stream, it.kvh, t_begin, t_end, ring, w.most, w.held, kLift, part);
+    if (owned) r.m = w.most, r.l = part[kPairs * D + lg];
+    const uint32_t rows = __ballot_sync(0xffffffffu, owned);
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+        if ((rows >> (4 * (2 * lt + c))) & 1u)
+#pragma unroll
+            for (int n = 0; n < W; ++n)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) r.o[4 * n + i / 2][2 * (i & 1) + c] = part[(2 * lt + c) * D + 8 * (W * lg + n) + i];
+    __syncwarp();
+}
 
 // One warp over the tiles [tile_a, tile_b) of an item, two at a time through its
 // ring of two stages. kFour (32-bit calls of up to four pairs a stream, passes of four): rows lg and
@@ -187,66 +157,18 @@ __device__ __forceinline__ void walk(const AttentionArgs<T> &g, const Item &it, 
         return (p0 ? 1 : 0) | (p1 ? 2 : 0);
     };
     float qv[NG][8];
-#pragma unroll
-    for (int j = 0; j < NG; ++j) {
-        if (live) {
-            load8(src + 32 * j + 8 * lt, qv[j], g.vec);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) qv[j][e] = 0.0f;
-        }
-    }
+    load_queries<T, D>(src, live, g.vec, qv);
     __syncwarp();
     int there = fetch(t_begin, ring), coming = 0;
 
     uint32_t q[2 * NG][4];
-    float unscale, slack;  // the scores' scale, kSlack before it
-    {
-        float top = 0.0f;
-#pragma unroll
-        for (int j = 0; j < NG; ++j)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(qv[j][e]));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // a power of two brings the largest below 2, into F16's range
-        int ex = top > 0.0f && top < INFINITY ? int(__float_as_uint(top) >> 23) - 127 : 0;
-        ex = min(max(ex, -100), 126);
-        const float down = __uint_as_float(uint32_t(127 - ex) << 23);
-        unscale = g.scale * __uint_as_float(uint32_t(127 + ex) << 23);
-        unscale = fminf(fmaxf(unscale, 1e-30f), 1e30f);
-        slack = kSlack / unscale;
-#pragma unroll
-        for (int j = 0; j < NG; ++j)
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const float q0 = qv[j][2 * s] * down, q1 = qv[j][2 * s + 1] * down;
-                const __half2 hi = __floats2half2_rn(q0, q1);
-                const float2 back = __half22float2(hi);
-                q[2 * j + s / 2][2 * (s & 1)] = h2u(hi);
-                q[2 * j + s / 2][2 * (s & 1) + 1] = h2u(__floats2half2_rn(q0 - back.x, q1 - back.y));
-            }
-    }
+    const float unscale = split_queries<D>(qv, g.scale, q), slack = kSlack / unscale;  // the scores' scale, kSlack before it
 #pragma unroll
     for (int i = 0; i < 4 * W; ++i) r.o[i][0] = r.o[i][1] = r.o[i][2] = r.o[i][3] = 0.0f;
     float m = -INFINITY, l = 0.0f, most = -INFINITY;
     r.bad = 0;
 
-    // this lane's places in a tile
-    const int key_at = (4 * (lg >> 1) + (lg & 1)) * (D / 2) + lt * (4 * NG);
-    const int key_scale_at = 16 * D + (4 * (lg >> 1) + (lg & 1)) * (2 * NG);
-    // row 4 lt + i of the values, its chunks as copy_tile put them; words of one chunk are n = 0
-    int value_at[D == 192 ? 4 : D == 128 ? 2 : 1][NS];
-#pragma unroll
-    for (int i = 0; i < (D == 192 ? 4 : D == 128 ? 2 : 1); ++i)
-#pragma unroll
-        for (int n = 0; n < NS; ++n) value_at[i][n] = 8 * D + (((4 * lt + i) * (D / 2) + 4 * (W * lg + n)) ^ (lt << 5));
-    auto value_row = [&](int i, int n) {
-        if constexpr (D == 64) return value_at[0][0] ^ (32 * i);
-        else if constexpr (D == 128) return value_at[i & 1][0] + 128 * (i >> 1);
-        else if constexpr (D == 192) return value_at[i][n];
-        else return value_at[0][0] + 128 * i;
-    };
+    const LanePlaces<D> at;  // this lane's places in a tile
     for (int t = t_begin; t < t_end; t += 2, there = coming) {
         const int t0 = 16 * t;
         const uint8_t *stage = ring + ((t - t_begin) & 2) * TB;
@@ -254,34 +176,10 @@ __device__ __forceinline__ void walk(const AttentionArgs<T> &g, const Item &it, 
         coming = fetch(t + 2, ring + ((t + 2 - t_begin) & 2) * TB);
         copy_wait<1>();
         __syncwarp();
-        float c[2][2][4];
-#pragma unroll
-        for (int zu = 0; zu < 4; ++zu) {
-            const uint8_t *at = stage + (zu >> 1) * TB + (zu & 1) * D;
-            uint32_t k[NG], ks[NG / 2];
-            load_words(k, at + key_at);
-            load_words(ks, stage + (zu >> 1) * TB + (zu & 1) * (4 * NG) + key_scale_at);
-#pragma unroll
-            for (int j = 0; j < NG; ++j) {
-                const __half2 both = u2h(ks[j / 2]), offs = __hmul2(both, __float2half2_rn(-24.0f));
-                const __half2 s = j & 1 ? __high2half2(both) : __low2half2(both);
-                const __half2 off = j & 1 ? __high2half2(offs) : __low2half2(offs);
-                if (j == 0) mma_first(c[zu >> 1][zu & 1], q[0], unpack<0>(k[0], s, off), unpack<1>(k[0], s, off));
-                else mma(c[zu >> 1][zu & 1], q[2 * j], unpack<0>(k[j], s, off), unpack<1>(k[j], s, off));
-                mma(c[zu >> 1][zu & 1], q[2 * j + 1], unpack<2>(k[j], s, off), unpack<3>(k[j], s, off));
-            }
-        }
-        uint2 vs[2][NS];
-#pragma unroll
-        for (int z = 0; z < 2; ++z)
-#pragma unroll
-            for (int n = 0; n < NS; ++n)
-                vs[z][n] = *reinterpret_cast<const uint2 *>(stage + z * TB + 17 * D + (W * lg + n) / 4 * 32 + 8 * lt);
         float s[2][4];
-#pragma unroll
-        for (int z = 0; z < 2; ++z)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[z][i] = c[z][i >> 1][i & 1] + c[z][i >> 1][2 + (i & 1)];
+        score_two<D>(stage, at, q, s);
+        uint2 vs[2][NS];
+        value_scales<D>(stage, vs);
         if (t0 < all_first || t0 + 31 > all_last || there != 3) {
 #pragma unroll
             for (int z = 0; z < 2; ++z)
@@ -355,43 +253,7 @@ __device__ __forceinline__ void walk(const AttentionArgs<T> &g, const Item &it, 
                     if (kFour && lg >= 4) hi[z][u] = lo[z][u];
                 }
             }
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-            uint32_t v[4][W];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (NS == 1) {
-                    load_words(v[i], stage + z * TB + value_row(i, 0));
-                } else {
-#pragma unroll
-                    for (int n = 0; n < NS; ++n)
-                        v[i][n] = *reinterpret_cast<const uint32_t *>(stage + z * TB + value_row(i, n));
-                }
-            }
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const uint2 sv = vs[z][NS == 3 ? w : 0];
-                const __half2 s01 = u2h(sv.x), s23 = u2h(sv.y), minus = __float2half2_rn(-24.0f);
-                const __half2 f01 = __hmul2(s01, minus), f23 = __hmul2(s23, minus);
-                const uint32_t lo01 = __byte_perm(v[0][w], v[1][w], 0x5410),
-                               hi01 = __byte_perm(v[0][w], v[1][w], 0x7632),
-                               lo23 = __byte_perm(v[2][w], v[3][w], 0x5410),
-                               hi23 = __byte_perm(v[2][w], v[3][w], 0x7632);
-                auto step = [&](float (&acc)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
-                    const uint32_t f[4] = {a0, a1, a2, a3};
-                    mma(acc, f, hi[z][0], hi[z][1]);
-                    if constexpr (kWide && !kFour) mma(acc, f, lo[z][0], lo[z][1]);
-                };
-                step(r.o[4 * w], unpack<0>(lo01, s01, f01), unpack<0>(hi01, s01, f01), unpack<0>(lo23, s23, f23),
-                     unpack<0>(hi23, s23, f23));
-                step(r.o[4 * w + 1], unpack<1>(lo01, s01, f01), unpack<1>(hi01, s01, f01), unpack<1>(lo23, s23, f23),
-                     unpack<1>(hi23, s23, f23));
-                step(r.o[4 * w + 2], unpack<2>(lo01, s01, f01), unpack<2>(hi01, s01, f01), unpack<2>(lo23, s23, f23),
-                     unpack<2>(hi23, s23, f23));
-                step(r.o[4 * w + 3], unpack<3>(lo01, s01, f01), unpack<3>(hi01, s01, f01), unpack<3>(lo23, s23, f23),
-                     unpack<3>(hi23, s23, f23));
-            }
-        }
+        add_values<D, kWide && !kFour>(stage, at, vs, hi, lo, r.o);
     }
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
@@ -405,40 +267,17 @@ __device__ __forceinline__ void walk(const AttentionArgs<T> &g, const Item &it, 
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
         const float largest = ex2(fmaf(most, unscale, kLift - (m == -INFINITY ? 0.0f : m) * unscale));
-        const bool owned = most > -INFINITY && l - largest < kOwned * largest;
-        uint32_t rows_owned = __ballot_sync(0xffffffffu, owned && lt == 0 && (!kFour || lg < 4));
-        while (rows_owned) {
-            const int from = __ffs(rows_owned) - 1, pr = from >> 2;
-            rows_owned &= rows_owned - 1;
-            const int p_pos = __shfl_sync(0xffffffffu, position, from), p_first = __shfl_sync(0xffffffffu, first, from);
-            // a token that is alone needs no second look
-            if (min(p_pos, 16 * t_end - 1) <= max(p_first, 16 * t_begin)) continue;
-            const float base = __shfl_sync(0xffffffffu, m * unscale, from) - kLift;
-            const T *qp = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), from));
-            float acc[NG], sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < NG; ++i) acc[i] = 0.0f;
-            for (int t = t_begin; t < t_end; ++t)
-                if (const uint8_t *tile = tile_at(t))
-                    sum += exact_tile<T, D>(qp, tile, 16 * t, p_first, p_pos, g.scale, base, acc);
-            if (lg == pr) l = sum;
-            __syncwarp();
-            float *scratch = reinterpret_cast<float *>(ring);
-#pragma unroll
-            for (int i = 0; i < NG; ++i) scratch[32 * i + lane] = acc[i];
-            __syncwarp();
-            if ((pr >> 1) == lt) {
-#pragma unroll
-                for (int w = 0; w < W; ++w)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float v = scratch[8 * (W * lg + w) + 2 * i + h];
-                            if (pr & 1) r.o[4 * w + i][2 * h + 1] = v;
-                            else r.o[4 * w + i][2 * h] = v;
-                        }
-            }
+        // a token that is alone needs no second look
+        const bool owned = most > -INFINITY && l - largest < kOwned * largest && (!kFour || lg < 4) &&
+                           min(position, 16 * t_end - 1) > max(first, 16 * t_begin);
+        if (__any_sync(0xffffffffu, owned)) {
+            // by way of memory, so that the sums' registers need not outlive the call
+            const Item again = it;
+            Sums<D> copy = r;
+            copy.m = m, copy.l = l;
+            look_again<T, D, kFour>(g, again, tile_a, tile_b, owned, ring, copy);
+            r = copy;
+            m = r.m, l = r.l;
         }
     }
     r.m = m * unscale;

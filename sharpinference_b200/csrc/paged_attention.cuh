@@ -1,5 +1,5 @@
 // What the kernels of attention over the paged 4-bit cache share: their
-// arguments, unpacking, and the exact pass over one pair's tokens.
+// arguments, unpacking, and a stream's share of the work.
 #pragma once
 
 #include "device_common.cuh"
@@ -44,39 +44,6 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
-}
-
-// One pair's tokens of one tile in FP32, by one warp: two lanes score a token,
-// then a lane adds the channels lane, lane + 32, ... Probabilities are
-// exp2(score - base); returns their sum.
-template <class T, int D>
-__device__ float exact_tile(const T *q, const uint8_t *tile, int t0, int first, int position, float scale, float base,
-                            float (&acc)[D / 32]) {
-    constexpr int NG = D / 32;
-    const int lane = threadIdx.x & 31, slot = lane >> 1, t = t0 + slot;
-    float s = 0.0f;
-    for (int w = 2 * (lane & 1); w < 2 * (lane & 1) + 2; ++w)
-        for (int j = 0; j < NG; ++j) {
-            const uint32_t word = reinterpret_cast<const uint32_t *>(tile)[slot * (D / 8) + w * NG + j];
-            const float ks = __half2float(reinterpret_cast<const __half *>(tile + 16 * D)[slot * NG + j]);
-            for (int e = 0; e < 8; ++e)
-                s = fmaf(ldf(q + 32 * j + 8 * w + e), ks * float(int((word >> (4 * (e >> 1) + 16 * (e & 1))) & 15u) - 8), s);
-        }
-    s += __shfl_xor_sync(0xffffffffu, s, 1);
-    float p = t >= first && t <= position ? exp2f(s * scale - base) : 0.0f;
-    for (int k = 0; k < 16; ++k) {
-        const float pk = __shfl_sync(0xffffffffu, p, 2 * k);
-        if (t0 + k < first || t0 + k > position) continue;
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            const uint32_t word = reinterpret_cast<const uint32_t *>(tile + 8 * D)[k * (D / 8) + 4 * i + lane / 8];
-            const float vs = __half2float(reinterpret_cast<const __half *>(tile + 17 * D)[i * 16 + k]);
-            acc[i] = fmaf(pk, vs * float(int((word >> (4 * ((lane & 7) >> 1) + 16 * (lane & 1))) & 15u) - 8), acc[i]);
-        }
-    }
-#pragma unroll
-    for (int o = 16; o > 1; o >>= 1) p += __shfl_xor_sync(0xffffffffu, p, o);
-    return p;
 }
 
 // A stream's share of the work: its rows make ceil(n * group / pairs) passes per

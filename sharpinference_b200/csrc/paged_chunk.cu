@@ -29,7 +29,7 @@
 #include <algorithm>
 
 #include "launch.cuh"
-#include "paged_attention.cuh"
+#include "paged_fragments.cuh"
 
 namespace si::kernels {
 namespace {
@@ -305,21 +305,60 @@ struct PairOf {
     }
 };
 
-// One row in FP32 by one warp: probabilities are exp2(score - base).
-template <class T, int D>
-__device__ __noinline__ void exact_row(const AttentionArgs<T> &g, const Place &at, int pair, float base) {
-    constexpr int NG = D / 32;
-    const PairOf<T> of(g, at, pair, D);
-    const int lane = threadIdx.x & 31;
-    float acc[NG], sum = 0.0f;
-#pragma unroll
-    for (int n = 0; n < NG; ++n) acc[n] = 0.0f;
-    for (int tok = of.first & ~15; tok <= of.position; tok += 16)
-        if (const uint8_t *tile = tile_of(g.a, at.stream, tok, at.kvh))
-            sum += exact_tile<T, D>(g.query + (at.sw.begin + of.row) * g.query_stride + int64_t(of.head) * D, tile, tok,
-                                    of.first, of.position, g.scale, base, acc);
-#pragma unroll
-    for (int n = 0; n < NG; ++n) stf(of.out + 32 * n + lane, sum != 0.0f ? acc[n] / sum : 0.0f);
+// Rows that one token owns, summed again by the NW warps of a block, eight at a time: of the pairs from `pair0` on that
+// have a bit in the `words` words `rows`, every `many`-th from the `which`-th on. The place's tokens are spread over the
+// warps, whose sums are added up in their order. `smem`: a ring for every warp, then its rows' maxima.
+template <int D, int NW>
+constexpr int owned_bytes() {
+    return NW * (4 * tile_bytes(D) + kPairs * 4);
+}
+template <class T, int D, int NW>
+__device__ __noinline__ void sum_owned(const AttentionArgs<T> &g, const Place &at, int pair0, const uint32_t *rows, int words,
+                                       const uint32_t *bad, int which, int many, uint8_t *smem) {
+    constexpr int kRing = 4 * tile_bytes(D), kStepTiles = kTokens / kTileTokens;
+    static_assert(kRing >= kPairs * (D + 1) * 4, "the ring takes a warp's sums");
+    float *most_of = reinterpret_cast<float *>(smem + NW * kRing);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lg = lane >> 2, lt = lane & 3;
+    uint8_t *ring = smem + warp * kRing;
+    const int tiles = at.steps * kStepTiles, share = (tiles + 2 * NW - 1) / (2 * NW) * 2;
+    const int begin = at.step0 * kStepTiles + min(warp * share, tiles), end = min(begin + share, (at.step0 + at.steps) * kStepTiles);
+    int total = 0;
+    for (int i = 0; i < words; ++i) total += __popc(rows[i]);
+    for (int done = which; done < total; done += kPairs * many) {
+        // lane group lg takes the row with done + lg * many owned ones before it
+        int left = done + lg * many, mine = -1;
+        for (int i = 0; i < words && mine < 0; ++i) {
+            const int n = __popc(rows[i]);
+            if (left < n) mine = 32 * i + int(__fns(rows[i], 0, left + 1));
+            left -= n;
+        }
+        const PairOf<T> of(g, at, pair0 + max(mine, 0), D);
+        const OwnedPair<T> p{g.query + (at.sw.begin + of.row) * g.query_stride + int64_t(of.head) * D, of.position, of.first,
+                             mine >= 0};
+        float us;
+        const Windows w = find_windows<T, D>(g.a, g.scale, p, at.stream, at.kvh, begin, end, ring, &us);
+        if (lt == 0) most_of[warp * kPairs + lg] = w.most;
+        __syncthreads();
+        float most = -INFINITY;
+        for (int i = 0; i < NW; ++i) most = fmaxf(most, most_of[i * kPairs + lg]);
+        float *part = reinterpret_cast<float *>(ring);
+        sum_windows<T, D>(g.a, g.scale, p, at.stream, at.kvh, begin, end, ring, most, w.below(most, us), kLift, part);
+        __syncthreads();
+        for (int pr = warp; pr < kPairs; pr += NW) {
+            const int r = __shfl_sync(0xffffffffu, mine, 4 * pr);
+            T *out = reinterpret_cast<T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(of.out), 4 * pr));
+            if (r < 0) continue;
+            float l = 0.0f;
+            for (int i = 0; i < NW; ++i) l += reinterpret_cast<const float *>(smem + i * kRing)[kPairs * D + pr];
+            const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+            for (int c = lane; c < D; c += 32) {
+                float o = 0.0f;
+                for (int i = 0; i < NW; ++i) o += reinterpret_cast<const float *>(smem + i * kRing)[pr * D + c];
+                stf(out + c, (bad[r] >> (c >> 5)) & 1u ? NAN : o * inv);
+            }
+        }
+        __syncthreads();
+    }
 }
 
 template <class T, int D, bool kCut>
@@ -332,6 +371,7 @@ __global__ void __launch_bounds__(Chunk<T, D>::kThreads, 1) paged_chunk_kernel(c
     __shared__ __align__(8) uint64_t k_full[2], v_full[2], s_full[G][2], p_full[G][2], pv_done[G][2];
     __shared__ uint32_t tmem_slot, mapped[8], poisoned[8];  // of the last eight steps: K runs ahead of the softmax by fewer
     __shared__ int found[2], slot_of;
+    __shared__ uint32_t owned_rows[kWide ? kSoftmax / 32 : 1], bad_of[kWide ? kSoftmax : 1];  // of rows that one token owns
     const PagedArgs &a = g.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_trigger();
@@ -449,6 +489,7 @@ __global__ void __launch_bounds__(Chunk<T, D>::kThreads, 1) paged_chunk_kernel(c
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
+    bool healthy = true;  // no wait of this thread's rows ran out
 
     if (warp >= C::kMmaWarp) {
         // ---- the products of a group: one elected thread issues ------------------------------------------
@@ -836,10 +877,14 @@ __global__ void __launch_bounds__(Chunk<T, D>::kThreads, 1) paged_chunk_kernel(c
         ok = !__any_sync(0xffffffffu, !ok);
         tc_fence_after();
         T *const out = PairOf<T>(g, at, pass * kBlockRows + tid, D).out;
-        bool owned = false;
-        if constexpr (kWide) {  // a row that one token owns: its small probabilities once more, in FP32
+        if constexpr (kWide) {  // rows that one token owns: a token that is alone needs no second look
             const float largest = ex2(fmaf(most, unscale, kLift - (m == -INFINITY ? 0.0f : m) * unscale));
-            owned = (!kCut || at.parts == 1) && out && most > -INFINITY && l - largest < kOwned * largest && min(position, any_last) > first;
+            const bool owned = (!kCut || at.parts == 1) && ok && out && most > -INFINITY && l - largest < kOwned * largest &&
+                               min(position, any_last) > first;
+            const uint32_t rows = __ballot_sync(0xffffffffu, owned);
+            if (lane == 0) owned_rows[warp] = rows;
+            bad_of[tid] = bad;
+            healthy = ok;
         }
         if (kCut && ok && at.parts > 1) {  // one part of the row's sums, for the join
             if (my_steps > 0) {
@@ -886,15 +931,16 @@ __global__ void __launch_bounds__(Chunk<T, D>::kThreads, 1) paged_chunk_kernel(c
                 __syncwarp();
             }
         }
-        __syncwarp();
-        if constexpr (kWide) {
-            uint32_t rows = __ballot_sync(0xffffffffu, ok && owned);
-            while (rows) {
-                const int from = __ffs(rows) - 1;
-                rows &= rows - 1;
-                const float p_base = __shfl_sync(0xffffffffu, m * unscale, from) - kLift;
+    }
+    if constexpr (kWide) {
+        static_assert(owned_bytes<D, C::kThreads / 32>() <= C::kSmem, "operands make room for the second look");
+        // all products are done where every row's last one is
+        if (!__syncthreads_or(!healthy)) {
+            uint32_t any = 0;
+            for (int i = 0; i < kSoftmax / 32; ++i) any |= owned_rows[i];
+            if (any) {
                 const Place copy = at;  // `at` itself stays in registers
-                exact_row<T, D>(g, copy, pass * kBlockRows + (tid & ~31) + from, p_base);
+                sum_owned<T, D, C::kThreads / 32>(g, copy, pass * kBlockRows, owned_rows, kSoftmax / 32, bad_of, 0, 1, q_tile);
             }
         }
     }
@@ -932,9 +978,9 @@ __global__ void __launch_bounds__(kRows) paged_chunk_join_kernel(const __grid_co
     const float *slot = g.parts + int64_t(item) * g.splits * C::kSlot;
     const float *stats = slot + kBlockRows * D + own * kRows + tid, *o = slot + own * (kRows * D) + tid * 4 + c * kRows;
     bool owned = false;
-    float top = -INFINITY;
+    uint32_t bad = 0;
     if (of.out) {
-        float most = -INFINITY;
+        float top = -INFINITY, most = -INFINITY;
 #pragma unroll 4
         for (int k = 0; k < at.parts; ++k) {
             top = fmaxf(top, __ldcg(stats + int64_t(k) * C::kSlot));
@@ -942,7 +988,6 @@ __global__ void __launch_bounds__(kRows) paged_chunk_join_kernel(const __grid_co
         }
         float l = 0.0f;
         float4 acc[kChannels / 4];
-        uint32_t bad = 0;
 #pragma unroll
         for (int j = 0; j < kChannels / 4; ++j) acc[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
@@ -970,13 +1015,17 @@ __global__ void __launch_bounds__(kRows) paged_chunk_join_kernel(const __grid_co
             }
         }
     }
-    if constexpr (C::kWide) {  // the first channels' block does an owned row alone
-        uint32_t rows = __ballot_sync(0xffffffffu, owned && c == 0);
-        while (rows) {
-            const int from = __ffs(rows) - 1;
-            rows &= rows - 1;
-            const float base = __shfl_sync(0xffffffffu, top, from) - kLift;
-            exact_row<T, D>(g, at, pair - (tid & 31) + from, base);
+    if constexpr (C::kWide) {  // owned rows go round the blocks of all channels
+        extern __shared__ __align__(128) uint8_t rings[];
+        __shared__ uint32_t owned_rows[kRows / 32], bad_of[kRows];
+        const uint32_t rows = __ballot_sync(0xffffffffu, owned);
+        if ((tid & 31) == 0) owned_rows[tid >> 5] = rows;
+        bad_of[tid] = bad;
+        if (__syncthreads_or(owned)) {
+            const Place whole =
+                place_at(g.a, g.group, g.window, kBlockRows, 1, found[0], found[1], item % g.a.kv_heads, 0);
+            sum_owned<T, D, kRows / 32>(g, whole, at.pass * kBlockRows + own * kRows, owned_rows, kRows / 32, bad_of,
+                                        int(blockIdx.y), int(gridDim.y), rings);
         }
     }
 }
@@ -997,7 +1046,8 @@ si_status launch(const AttentionArgs<T> &all, void *stream) {
             launch_pdl("paged-attention", paged_chunk_kernel<T, D, true>, grid, block, Chunk<T, D>::kSmem, 1, stream, g))
         return e;
     return launch_pdl("paged-attention", paged_chunk_join_kernel<T, D>,
-                      dim3(unsigned(items) * Chunk<T, D>::kGroups, D / 16), dim3(kRows), 0, 1, stream, g);
+                      dim3(unsigned(items) * Chunk<T, D>::kGroups, D / 16), dim3(kRows),
+                      Chunk<T, D>::kWide ? owned_bytes<D, kRows / 32>() : 0, 1, stream, g);
 }
 
 template <class T>

@@ -223,7 +223,7 @@ template <class T, int VEC, int kThreads>
 si_status launch(LogitArgs<T> &g, int64_t rows, void *stream) {
     constexpr int kMaxChunk = kTokens * kThreads;
     // as many blocks to a row (16 is beyond the portable 8) as run at once: a second wave would pay every block's
-    // start again (128 rows of 100352: 40.8 us, 47.0 with four blocks to a row; one row of 200064: 12.1 us, 17 with 8)
+    // start again (128 rows of 100352: 39.5 us, 45.6 with four blocks to a row; one row of 200064: 8.5 us, 11.4 with 8)
     const int64_t room = int64_t(1024 / kThreads) * device_sm_count() / rows;
     const int64_t want = std::min<int64_t>(room, (g.vocab + 2047) / 2048);
     const int cluster = int(want >= 16 ? 16 : std::max<int64_t>(1, std::min<int64_t>(want, 8)));

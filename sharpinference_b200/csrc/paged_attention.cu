@@ -12,16 +12,19 @@
 //   values  C[16 channels, 8] += A[16 channels, 16 tokens] B[16 tokens, 8]:
 //     a score's place in C is its probability's place in B, so probabilities
 //     never leave their lanes; F32 calls add the product with what rounding
-//     them to F16 left over.
+//     them to F16 left over. F16 calls leave that out: it is up to 2^-11 of a
+//     probability, no more than the rounding of their outputs loses (relative
+//     error of 16 streams of 2047 tokens 2.3e-4 .. 2.6e-4, rounding the outputs
+//     alone 2.1e-4).
 // The tiles of 16 tokens of all streams, heads and passes form one line that is
 // cut evenly over the warps of the grid, so uneven lengths balance. A warp walks
 // its cut with running maxima that move only when a score exceeds them by 2^2,
 // the next two tiles on their way into its ring; items that a cut divides are put together
 // in shared memory once per block, and over the blocks by the last to arrive.
 // Measured: 64 streams of up to 4096 tokens (40 query, 10 key/value heads of 128,
-// F32) 72 us, 3.2 TB/s: near half each of the ALU, FMA and tensor pipes at the
+// F32) 71 us, 3.2 TB/s: near half each of the ALU, FMA and tensor pipes at the
 // three warps a scheduler that the registers allow. One stream of 32768 tokens (24, 8
-// heads) 22.6 us, of which the tiles take 11.5.
+// heads) 21.3 us, of which the tiles take about half.
 // F16 probabilities end 2^-37 below a row's largest. In an F32 row that
 // one token owns (all others together below 2^-16 of it) the channels in which
 // that token's value is 0 consist of such small ones, so a warp that meets
@@ -39,9 +42,9 @@ namespace {
 using namespace si::dev;
 
 // Pairs of a row and a query head of a stream and key/value head; more go to paged_chunk.cu. Measured with 4
-// key/value heads of 128, us here / there: 16 streams of 2047 tokens, F32 32 pairs 37/49, 64 pairs 56/65, 96 pairs
-// 78/67, F16 24 pairs 30/36, 32 pairs 35/35, 44 pairs 46/36; 64 of 1500, F32 32 pairs 81/101, 44 pairs 110/102, F16
-// 74/72 and 100/73; one of 32768, F32 64 pairs 57/72, 96 pairs 79/74, F16 44 pairs 41/55, 96 pairs 71/56.
+// key/value heads of 128, us here / there: 16 streams of 2047 tokens, F32 32 pairs 37/51, 64 pairs 57/66, 96 pairs
+// 74/68, F16 24 pairs 30/36, 32 pairs 36/35, 44 pairs 44/35; 64 of 1500, F32 32 pairs 77/104, 44 pairs 104/106, F16
+// 72/71 and 97/72; one of 32768, F32 64 pairs 55/53, 96 pairs 73/53, F16 44 pairs 42/54, 96 pairs 69/55.
 constexpr int kFewPairs = 32;
 constexpr float kSlack = 2.0f;    // log2 of what a score may exceed the running maximum by
 constexpr float kLift = 13.0f;    // log2 of a probability at the maximum: F16 keeps more small ones
@@ -107,7 +110,7 @@ __device__ __noinline__ void look_again(const AttentionArgs<T> &g, const Item &i
 // ring of two stages. kFour (32-bit calls of up to four pairs a stream, passes of four): rows lg and
 // lg + 4 of the scores are the same pair, and the probabilities' columns lg + 4
 // hold what rounding left of columns lg, so that one product does for both (64
-// streams of 4 pairs: 86.2 us against 90.0).
+// streams of 4 pairs: 70.9 us against 75.1).
 template <class T, int D, bool kFour>
 __device__ __forceinline__ void walk(const AttentionArgs<T> &g, const Item &it, int tile_a, int tile_b, uint8_t *ring,
                                      Sums<D> &r) {

@@ -12,17 +12,19 @@
 // once for both groups: two warps write K as [token][channel], four V
 // transposed as [channel][token] (eight tokens of one word give eight 16-byte
 // runs), both in the 128-byte swizzled layout. F32 queries are two F16 numbers,
-// products with both added in the same accumulator. Running maxima move only
+// products with both added in the same accumulator; F16 calls round probabilities
+// to one F16 number (relative error of 4096 rows on 8192 tokens 2.7e-4, of which
+// rounding the outputs is 2.1e-4). Running maxima move only
 // when a score exceeds them by 2^7; then the row's O is scaled in tensor memory.
 // One group's exponentials run under the other's products. Blocks start with
 // the rows that see most. Measured: 4096 rows on 8192 tokens (24 query, 8
-// key/value heads of 128) F16 389 us, 0.79 PFLOP/s; F32, 3 chunks of up to 777
-// rows on 1500 tokens (40, 10 heads) 119 us.
+// key/value heads of 128) F16 391 us, 0.79 PFLOP/s; F32, 3 chunks of up to 777
+// rows on 1500 tokens (40, 10 heads) 120 us.
 //
 // While there are fewer blocks than SMs, each block's tokens are cut into parts
 // of two steps or more, for as many blocks as fit; a part's sums lie in its slot of
 // the workspace and a second launch joins them. 16 rows of 4 heads a key/value
-// head on 32768 tokens, 4 key/value heads: 66 us, 758 uncut; on 4096: 34 and 105.
+// head on 32768 tokens, 4 key/value heads, F32: 50 us, 758 uncut; on 4096: 27 and 105.
 //
 // Every wait is bounded (device error word, no trap): a thread whose wait runs
 // out leaves its loop, and the block frees its tensor memory and ends.
@@ -278,8 +280,9 @@ __device__ __forceinline__ Place place_at(const PagedArgs &a, int group, int win
     p.any_last = min(p.sw.length - p.sw.rows + row_last, capacity - 1);
     p.any_first = window ? max(0, p.sw.length - p.sw.rows + row_first - window + 1) : 0;
     const int step0 = p.any_first / kTokens, steps = p.any_last < p.any_first ? 0 : p.any_last / kTokens - step0 + 1;
-    // a part's steps against the parts' join: the best number grows with the root of the steps (times of 64 pairs of
-    // F32 on 16, 64, 128 steps: 26, 36, 47 us with parts of 4 steps, 29, 36, 43 with parts of 8)
+    // a part's steps against the parts' join: the best number grows with the root of the steps (us of 64 pairs on 16,
+    // 64, 128 steps: F16 20, 27, 32; with parts of 4 steps 19, 27, 37, of 8 22, 26, 32; F32 20, 27, 30; 20, 24, 28; 27,
+    // 28, 30)
     p.parts = max(min(min(splits, int(sqrtf(2.0f * float(steps)))), steps / 2), 1);
     const int from = int(int64_t(steps) * part / p.parts);
     p.step0 = step0 + from;

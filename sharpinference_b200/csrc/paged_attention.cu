@@ -22,7 +22,7 @@
 // the next two tiles on their way into its ring; items that a cut divides are put together
 // in shared memory once per block, and over the blocks by the last to arrive.
 // Measured: 64 streams of up to 4096 tokens (40 query, 10 key/value heads of 128,
-// F32) 71 us, 3.2 TB/s: near half each of the ALU, FMA and tensor pipes at the
+// F32) 72 us, 3.2 TB/s: near half each of the ALU, FMA and tensor pipes at the
 // three warps a scheduler that the registers allow. One stream of 32768 tokens (24, 8
 // heads) 21.3 us, of which the tiles take about half.
 // F16 probabilities end 2^-37 below a row's largest. In an F32 row that
@@ -48,6 +48,11 @@ using namespace si::dev;
 constexpr int kFewPairs = 32;
 constexpr float kSlack = 2.0f;    // log2 of what a score may exceed the running maximum by
 constexpr float kLift = 13.0f;    // log2 of a probability at the maximum: F16 keeps more small ones
+// The products truncate what they add up. F32 calls take the sums out of the accumulators every kFlush tiles and add
+// them up rounded, in memory of their own (32768 tokens that one warp walks, values of one sign: off by 1.3e-4 of the
+// output without, 1.9e-6 so; mixed signs 4.2e-5 and 1.4e-6). 64 streams of up to 4096 tokens, 92
+// tiles a warp: 71.1 us without, 72.0 so, 71.6 with 64 tiles.
+constexpr int kFlush = 32;
 template <bool kFour>
 constexpr int pass_pairs() {  // where rows or columns of the products hold a pair twice (`walk`)
     return kFour ? kPairs / 2 : kPairs;
@@ -80,8 +85,8 @@ struct Item {
 
 // Sums of those pairs of an item anew that one token owns (the maxima before their scale).
 template <class T, int D, bool kFour>
-__device__ __noinline__ void look_again(const AttentionArgs<T> &g, const Item &it, int tile_a, int tile_b, bool owned, uint8_t *ring,
-                                        Sums<D> &r) {
+__device__ __noinline__ void look_again(const AttentionArgs<T> &g, const Item &it, int tile_a, int tile_b, bool owned,
+                                        uint8_t *ring, Sums<D> &r) {
     constexpr int W = D / 64;
     const int lane = threadIdx.x & 31, lg = lane >> 2, lt = lane & 3;
     const int pair = it.pass * pass_pairs<kFour>() + lg, row = pair / g.group;
@@ -110,7 +115,7 @@ __device__ __noinline__ void look_again(const AttentionArgs<T> &g, const Item &i
 // ring of two stages. kFour (32-bit calls of up to four pairs a stream, passes of four): rows lg and
 // lg + 4 of the scores are the same pair, and the probabilities' columns lg + 4
 // hold what rounding left of columns lg, so that one product does for both (64
-// streams of 4 pairs: 70.9 us against 75.1).
+// streams of 4 pairs: 70.9 us against 75.1, both without the sums put away).
 template <class T, int D, bool kFour>
 __device__ __forceinline__ void walk(const AttentionArgs<T> &g, const Item &it, int tile_a, int tile_b, uint8_t *ring,
                                      Sums<D> &r) {
@@ -170,93 +175,118 @@ __device__ __forceinline__ void walk(const AttentionArgs<T> &g, const Item &it, 
     for (int i = 0; i < 4 * W; ++i) r.o[i][0] = r.o[i][1] = r.o[i][2] = r.o[i][3] = 0.0f;
     float m = -INFINITY, l = 0.0f, most = -INFINITY;
     r.bad = 0;
-
+    float flushed = 1.0f;  // how far the maximum has moved since sums were put away
+    bool begun = false;    // some are
+    auto held_at = [&](int i) {
+        return g.held + (int64_t(blockIdx.x) * warps<D>() + (threadIdx.x >> 5)) * (4 * W * 32) + 32 * i + lane;
+    };
     const LanePlaces<D> at;  // this lane's places in a tile
-    for (int t = t_begin; t < t_end; t += 2, there = coming) {
-        const int t0 = 16 * t;
-        const uint8_t *stage = ring + ((t - t_begin) & 2) * TB;
-        __syncwarp();  // the other stage's readers are done
-        coming = fetch(t + 2, ring + ((t + 2 - t_begin) & 2) * TB);
-        copy_wait<1>();
-        __syncwarp();
-        float s[2][4];
-        score_two<D>(stage, at, q, s);
-        uint2 vs[2][NS];
-        value_scales<D>(stage, vs);
-        if (t0 < all_first || t0 + 31 > all_last || there != 3) {
+    for (int t = t_begin;;) {
+        const int stop = kWide ? min(t + kFlush, t_end) : t_end;
+        for (; t < stop; t += 2, there = coming) {
+            const int t0 = 16 * t;
+            const uint8_t *stage = ring + ((t - t_begin) & 2) * TB;
+            __syncwarp();  // the other stage's readers are done
+            coming = fetch(t + 2, ring + ((t + 2 - t_begin) & 2) * TB);
+            copy_wait<1>();
+            __syncwarp();
+            float s[2][4];
+            score_two<D>(stage, at, q, s);
+            uint2 vs[2][NS];
+            value_scales<D>(stage, vs);
+            if (t0 < all_first || t0 + 31 > all_last || there != 3) {
+#pragma unroll
+                for (int z = 0; z < 2; ++z)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int token = t0 + 16 * z + 4 * lt + i;
+                        const bool none = !((there >> z) & 1);
+                        if (none || token < first || token > position) s[z][i] = -INFINITY;
+                        if (none || token < any_first || token > any_last) {  // whatever is there: zeros
+#pragma unroll
+                            for (int n = 0; n < NS; ++n) {
+                                uint32_t &half_pair = i < 2 ? vs[z][n].x : vs[z][n].y;
+                                half_pair &= i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+                            }
+                        }
+                    }
+            }
+            uint32_t odd = 0;
+#pragma unroll
+            for (int n = 0; n < 2 * NS; ++n) odd |= not_finite(vs[n & 1][n >> 1].x) | not_finite(vs[n & 1][n >> 1].y);
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
+            if constexpr (kWide) most = fmaxf(most, top);
+            // rare: a NaN among the values' scales, a score above its maximum
+            if (__any_sync(0xffffffffu, (odd & 0x80008000u) || top > m + slack)) {
+                if (__any_sync(0xffffffffu, odd & 0x80008000u)) {
+                    // a NaN in the cache reaches the pairs that see its token, not the others of the product
+                    for (int i = 0; i < 32; ++i)
+                        if ((there >> (i >> 4)) & 1)
+                            for (int j = 0; j < NG; ++j) {
+                                const uint32_t v =
+                                    reinterpret_cast<const uint16_t *>(stage + (i >> 4) * TB + 17 * D)[j * 16 + (i & 15)];
+                                if ((v & 0x7C00u) == 0x7C00u && t0 + i >= first && t0 + i <= position) r.bad |= 1u << j;
+                            }
+#pragma unroll
+                    for (int n = 0; n < 4 * NS; ++n) {
+                        uint2 &pair_of = vs[n & 1][n >> 2];
+                        uint32_t &h = n & 2 ? pair_of.y : pair_of.x;
+                        if ((h & 0x7C00u) == 0x7C00u) h &= 0xFFFF0000u;
+                        if ((h & 0x7C000000u) == 0x7C000000u) h &= 0x0000FFFFu;
+                    }
+                }
+                // a pair's maximum moves by its own scores alone
+                float up = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 2));
+                const bool moves = up > m + slack;
+                const float alpha = moves ? ex2((m - up) * unscale) : 1.0f;
+                if (moves) m = up;
+                l *= alpha;
+                flushed *= alpha;
+                const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * lt), a1 = __shfl_sync(0xffffffffu, alpha, 8 * lt + 4);
+#pragma unroll
+                for (int i = 0; i < 4 * W; ++i) {
+                    r.o[i][0] *= a0, r.o[i][2] *= a0;
+                    r.o[i][1] *= a1, r.o[i][3] *= a1;
+                }
+            }
+            const float lift = kLift - (m == -INFINITY ? 0.0f : m) * unscale;
+            uint32_t hi[2][2], lo[2][2];
 #pragma unroll
             for (int z = 0; z < 2; ++z)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int token = t0 + 16 * z + 4 * lt + i;
-                    const bool none = !((there >> z) & 1);
-                    if (none || token < first || token > position) s[z][i] = -INFINITY;
-                    if (none || token < any_first || token > any_last) {  // whatever is there: zeros
-#pragma unroll
-                        for (int n = 0; n < NS; ++n) {
-                            uint32_t &half_pair = i < 2 ? vs[z][n].x : vs[z][n].y;
-                            half_pair &= i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-                        }
+                for (int u = 0; u < 2; ++u) {
+                    const float e0 = ex2(fmaf(s[z][2 * u], unscale, lift)), e1 = ex2(fmaf(s[z][2 * u + 1], unscale, lift));
+                    l += e0 + e1;
+                    const __half2 h = __floats2half2_rn(e0, e1);
+                    hi[z][u] = h2u(h);
+                    if constexpr (kWide) {
+                        const float2 f = __half22float2(h);
+                        lo[z][u] = h2u(__floats2half2_rn(e0 - f.x, e1 - f.y));
+                        if (kFour && lg >= 4) hi[z][u] = lo[z][u];
                     }
                 }
+            add_values<D, kWide && !kFour>(stage, at, vs, hi, lo, r.o);
         }
-        uint32_t odd = 0;
-#pragma unroll
-        for (int n = 0; n < 2 * NS; ++n) odd |= not_finite(vs[n & 1][n >> 1].x) | not_finite(vs[n & 1][n >> 1].y);
-        float top = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
-        if constexpr (kWide) most = fmaxf(most, top);
-        // rare: a NaN among the values' scales, a score above its maximum
-        if (__any_sync(0xffffffffu, (odd & 0x80008000u) || top > m + slack)) {
-            if (__any_sync(0xffffffffu, odd & 0x80008000u)) {
-                // a NaN in the cache reaches the pairs that see its token, not the others of the product
-                for (int i = 0; i < 32; ++i)
-                    if ((there >> (i >> 4)) & 1)
-                        for (int j = 0; j < NG; ++j) {
-                            const uint32_t v =
-                                reinterpret_cast<const uint16_t *>(stage + (i >> 4) * TB + 17 * D)[j * 16 + (i & 15)];
-                            if ((v & 0x7C00u) == 0x7C00u && t0 + i >= first && t0 + i <= position) r.bad |= 1u << j;
-                        }
-#pragma unroll
-                for (int n = 0; n < 4 * NS; ++n) {
-                    uint2 &pair_of = vs[n & 1][n >> 2];
-                    uint32_t &h = n & 2 ? pair_of.y : pair_of.x;
-                    if ((h & 0x7C00u) == 0x7C00u) h &= 0xFFFF0000u;
-                    if ((h & 0x7C000000u) == 0x7C000000u) h &= 0x0000FFFFu;
-                }
-            }
-            // a pair's maximum moves by its own scores alone
-            float up = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 2));
-            const bool moves = up > m + slack;
-            const float alpha = moves ? ex2((m - up) * unscale) : 1.0f;
-            if (moves) m = up;
-            l *= alpha;
-            const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * lt), a1 = __shfl_sync(0xffffffffu, alpha, 8 * lt + 4);
+        if (kWide && begun) {
+            const float f0 = __shfl_sync(0xffffffffu, flushed, 8 * lt), f1 = __shfl_sync(0xffffffffu, flushed, 8 * lt + 4);
 #pragma unroll
             for (int i = 0; i < 4 * W; ++i) {
-                r.o[i][0] *= a0, r.o[i][2] *= a0;
-                r.o[i][1] *= a1, r.o[i][3] *= a1;
+                const float4 y = __ldcg(held_at(i));
+                r.o[i][0] = fmaf(y.x, f0, r.o[i][0]), r.o[i][1] = fmaf(y.y, f1, r.o[i][1]);
+                r.o[i][2] = fmaf(y.z, f0, r.o[i][2]), r.o[i][3] = fmaf(y.w, f1, r.o[i][3]);
             }
         }
-        const float lift = kLift - (m == -INFINITY ? 0.0f : m) * unscale;
-        uint32_t hi[2][2], lo[2][2];
+        if (t >= t_end) break;
 #pragma unroll
-        for (int z = 0; z < 2; ++z)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const float e0 = ex2(fmaf(s[z][2 * u], unscale, lift)), e1 = ex2(fmaf(s[z][2 * u + 1], unscale, lift));
-                l += e0 + e1;
-                const __half2 h = __floats2half2_rn(e0, e1);
-                hi[z][u] = h2u(h);
-                if constexpr (kWide) {
-                    const float2 f = __half22float2(h);
-                    lo[z][u] = h2u(__floats2half2_rn(e0 - f.x, e1 - f.y));
-                    if (kFour && lg >= 4) hi[z][u] = lo[z][u];
-                }
-            }
-        add_values<D, kWide && !kFour>(stage, at, vs, hi, lo, r.o);
+        for (int i = 0; i < 4 * W; ++i) {
+            __stcg(held_at(i), make_float4(r.o[i][0], r.o[i][1], r.o[i][2], r.o[i][3]));
+            r.o[i][0] = r.o[i][1] = r.o[i][2] = r.o[i][3] = 0.0f;
+        }
+        begun = true;
+        flushed = 1.0f;
     }
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
@@ -717,17 +747,23 @@ si_status launch_size(const AttentionArgs<T> &g, void *stream) {
     }
 }
 
+// Bytes of the blocks' parts (two to a block), then of the sums that their warps put away.
+uint64_t part_bytes(int head_size) { return uint64_t(device_sm_count()) * 2 * kPairs * (uint64_t(head_size) + 2) * 4; }
+uint64_t held_bytes(int head_size) {
+    return uint64_t(device_sm_count()) * (head_size <= 128 ? warps<128>() : warps<256>()) * kPairs * uint64_t(head_size) * 4;
+}
+
 template <class T>
 si_status run(const PagedArgs &a, const PagedAttention &q, void *stream) {
     const int capacity = a.table_width << a.page_shift;
+    uint8_t *const parts = static_cast<uint8_t *>(q.workspace) + ticket_bytes();
     const AttentionArgs<T> g{a, static_cast<const T *>(q.query), static_cast<T *>(q.output), q.query_stride,
                              q.output_stride, q.query_heads, q.query_heads / a.kv_heads,
                              q.window < capacity ? q.window : 0, 2, q.scale * 1.44269504088896340736f,
                              whole8<T>(q.query, q.query_stride * int64_t(sizeof(T))),
                              whole8<T>(q.output, q.output_stride * int64_t(sizeof(T))),
-                             static_cast<uint32_t *>(q.workspace),
-                             reinterpret_cast<float *>(static_cast<uint8_t *>(q.workspace) + ticket_bytes()),
-                             device_sm_count(), 1};
+                             static_cast<uint32_t *>(q.workspace), reinterpret_cast<float *>(parts),
+                             reinterpret_cast<float4 *>(parts + part_bytes(a.head_size)), device_sm_count(), 1};
     if (int64_t(q.max_rows) * g.group > kFewPairs) return paged_chunk_attention(g, stream);
     if (sizeof(T) == 4 && int64_t(q.max_rows) * g.group <= pass_pairs<true>()) return launch_size<T, sizeof(T) == 4>(g, stream);
     return launch_size<T, false>(g, stream);
@@ -737,7 +773,7 @@ si_status run(const PagedArgs &a, const PagedAttention &q, void *stream) {
 
 uint64_t paged_attention_workspace(const PagedArgs &a, int64_t, int max_rows, int query_heads) {
     if (int64_t(max_rows) * (query_heads / a.kv_heads) > kFewPairs) return ticket_bytes() + paged_chunk_workspace(a.head_size);
-    return ticket_bytes() + uint64_t(device_sm_count()) * 2 * kPairs * (uint64_t(a.head_size) + 2) * 4;
+    return ticket_bytes() + part_bytes(a.head_size) + held_bytes(a.head_size);
 }
 
 si_status paged_attention(const PagedArgs &a, uint32_t type, const PagedAttention &q, void *stream) {

@@ -21,6 +21,7 @@ struct AttentionArgs {
     bool vec, vec_out;  // whole accesses of eight: query rows, output rows
     uint32_t *tickets;  // [slots], zero between calls
     float *parts;
+    float4 *held;       // [blocks][warps][4 words of a lane's values][lanes]: sums that left a warp's accumulators
     int slots;          // SMs
     int splits;         // parts of a block's tokens (prompt chunks)
 };

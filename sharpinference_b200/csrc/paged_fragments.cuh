@@ -226,6 +226,7 @@ __device__ __forceinline__ void add_values(const uint8_t *stage, const LanePlace
 // walk over the scores and one for every window that holds a token, for eight pairs together; calls whose rows are all
 // owned, us against the same call with ordinary scores: 64 streams of up to 4096 tokens 485 / 79, one of 32768 99 / 26,
 // three chunks of up to 777 rows 2200 / 126, 16 rows on 32768 tokens 1990 / 57 (213000 with a row to a warp in FP32).
+// The sums stay in their accumulators: what truncation takes off them is a small part of 2^-16 of a row.
 constexpr int kWindows = 7;
 constexpr float kWindowBits = 17.0f, kWindowLift = 14.0f;  // log2 of a window's width, of its largest probability
 

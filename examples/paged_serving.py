@@ -6,7 +6,8 @@ side; si_paged_rope_kv_append stores their keys and values in the requests'
 pages, si_paged_attention reads them, and si_process_logits applies each
 request's penalties, biases and grammar mask to its logits and picks the next
 token. Pages are taken from a free list as requests grow and go back when they
-end, and a waiting request takes the slot that became free.
+end. A waiting request takes a slot that became free once the pool has room for
+it at its full length, beside those that are being served.
 
     python examples/paged_serving.py [--requests 6] [--slots 4] [--tokens 24]
 """
@@ -57,7 +58,7 @@ class PagedServer:
     def __init__(self, cfg, weights, slots, pages, page_size=64, chunk=512):
         if cfg["embedding_type"] != native.F16:
             raise native.ArgumentError("the batched embedding lookup takes an F16 table.")
-        self.cfg, self.slots, self.page_size, self.chunk = cfg, slots, page_size, chunk
+        self.cfg, self.slots, self.pages, self.page_size, self.chunk = cfg, slots, pages, page_size, chunk
         self.weights = {n: torch.from_numpy(np.array(w)).cuda() for n, w in weights.items()}
         rotary = cfg["rotary_size"]
         self.frequencies = torch.from_numpy(
@@ -78,8 +79,10 @@ class PagedServer:
         self.workspace = torch.zeros(need, dtype=torch.uint8, device="cuda")
 
     def submit(self, request: Request):
-        if not 0 < len(request.prompt) <= self.cfg["context"] - request.new_tokens:
+        if request.new_tokens < 1 or not 0 < len(request.prompt) <= self.cfg["context"] - request.new_tokens:
             raise native.ArgumentError("a request's tokens have to fit the context.")
+        if self._pages(request) > self.pages:
+            raise native.ArgumentError("a request's tokens have to fit the pool.")
         self.waiting.append(request)
 
     def run(self):
@@ -88,11 +91,21 @@ class PagedServer:
             self.step()
 
     # ---- pages ---------------------------------------------------------------------------
+    def _pages(self, request):
+        """Pages of a request at its full length; the token picked last is never written."""
+        return (len(request.prompt) + request.new_tokens - 1 + self.page_size - 1) // self.page_size
+
+    def _admit(self):
+        for slot in range(self.slots):
+            if self.active[slot] is None and self.waiting:
+                taken = sum(self._pages(r) for r in self.active if r)
+                if taken + self._pages(self.waiting[0]) > self.pages:
+                    return
+                self.active[slot] = self.waiting.pop(0)
+
     def _grow(self, slot, tokens):
         for page in range((tokens + self.page_size - 1) // self.page_size):
             if self.table[slot, page] < 0:
-                if not self.free:
-                    raise native.OutOfMemoryError("no page is free.")
                 self.table[slot, page] = self.free.pop()
 
     def _release(self, slot):
@@ -102,9 +115,7 @@ class PagedServer:
 
     # ---- one step ------------------------------------------------------------------------
     def step(self):
-        for slot in range(self.slots):
-            if self.active[slot] is None and self.waiting:
-                self.active[slot] = self.waiting.pop(0)
+        self._admit()
         rows = [r.next_rows(self.chunk) if r else np.empty(0, np.int32) for r in self.active]
         lengths = [r.held + len(t) if r else 0 for r, t in zip(self.active, rows)]
         for slot, r in enumerate(self.active):

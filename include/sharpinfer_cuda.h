@@ -497,9 +497,9 @@ si_status si_paged_kv_gather(const si_paged_cache *cache, uint32_t type, const i
  * 2048, F32, 24 query and 8 key/value heads of 128: 276 us, apart 60 + 53; one
  * row on 32768 tokens beside that chunk 388 us, apart 22 + 55).
  * Sums and softmax statistics are FP32. F16 calls hold probabilities as F16
- * numbers, which costs about what rounding the output does, and their sums are
- * truncated (values of one sign lose up to 1.8e-4 over 32768 tokens, 7e-4 over
- * 131072). F32 calls take a few
+ * numbers, which costs about what rounding the output does, and prompt chunks'
+ * sums are truncated (values of one sign lose up to 1.8e-4 over 32768 tokens,
+ * 7e-4 over 131072). F32 calls take a few
  * times as long where one token holds nearly all of a row's weight.
  * The keys and values of the rows themselves must have been appended.
  * `workspace`: device scratch of si_paged_attention_workspace_bytes(...),

@@ -51,8 +51,9 @@ constexpr float kLift = 13.0f;    // log2 of a probability at the maximum: F16 k
 // The products truncate what they add up. F32 calls take the sums out of the accumulators every kFlush tiles and add
 // them up rounded, in memory of their own (32768 tokens that one warp walks, values of one sign: off by 1.3e-4 of the
 // output without, 1.9e-6 so; mixed signs 4.2e-5 and 1.4e-6). 64 streams of up to 4096 tokens, 92
-// tiles a warp: 71.1 us without, 72.0 so, 71.6 with 64 tiles.
-constexpr int kFlush = 32;
+// tiles a warp: 71.1 us without, 72.0 so, 71.6 with 64 tiles. F16 calls do so every 8192 tokens (131072 tokens of values
+// of one sign: off by 5.2e-4 without, 7e-5 so; their rounding 2.1e-4).
+constexpr int kFlush = 32, kFlushHalf = 512;
 template <bool kFour>
 constexpr int pass_pairs() {  // where rows or columns of the products hold a pair twice (`walk`)
     return kFour ? kPairs / 2 : kPairs;
@@ -182,7 +183,7 @@ __device__ __forceinline__ void walk(const AttentionArgs<T> &g, const Item &it, 
     };
     const LanePlaces<D> at;  // this lane's places in a tile
     for (int t = t_begin;;) {
-        const int stop = kWide ? min(t + kFlush, t_end) : t_end;
+        const int stop = min(t + (kWide ? kFlush : kFlushHalf), t_end);
         for (; t < stop; t += 2, there = coming) {
             const int t0 = 16 * t;
             const uint8_t *stage = ring + ((t - t_begin) & 2) * TB;
@@ -270,7 +271,7 @@ __device__ __forceinline__ void walk(const AttentionArgs<T> &g, const Item &it, 
                 }
             add_values<D, kWide && !kFour>(stage, at, vs, hi, lo, r.o);
         }
-        if (kWide && begun) {
+        if (begun) {
             const float f0 = __shfl_sync(0xffffffffu, flushed, 8 * lt), f1 = __shfl_sync(0xffffffffu, flushed, 8 * lt + 4);
 #pragma unroll
             for (int i = 0; i < 4 * W; ++i) {

@@ -76,3 +76,19 @@ def test_long_sums_whose_maxima_move(torch):
         pick = np.concatenate([np.arange(b * rows, b * rows + rows) for b in few])
         want, weight, reach = ref.attention(one, q[pick], [rows] * 4, heads, d ** -0.5)
         assert (np.abs(got[pick] - want) <= ref.attention_bound(one, weight, reach, want, False)).all()
+
+
+def test_long_sums_of_many_f16_streams(torch):
+    """131072 tokens, sums put away every 8192: 512 products lose at most 5.25 units each of a sum that grows from nothing,
+    672 in the mean; probabilities round by up to 2^-11, a quarter of that in the mean of many."""
+    d, streams, length, ps = 128, 1900, 131072, 256
+    s = ref.Streams(OneSign(d, ps, None), [length], 1, d, ps)
+    keys, values = (torch.from_numpy(x[0][:, 0]).cuda() for x in (s.keys, s.values))
+    s.table, s.lengths = np.repeat(s.table, streams, 0), [length] * streams
+    q = (0.1 + 1e-3 * np.random.default_rng(1).standard_normal((streams, d))).astype(np.float16)
+    got = torch.from_numpy(Device(torch, s).attend(q, [1] * streams, 1, d ** -0.5, type=native.F16)).cuda().double()
+    few = torch.arange(0, streams, 90, device="cuda")
+    x = torch.from_numpy(q.astype(np.float64)).cuda()[few] @ keys.T * d ** -0.5
+    off = got[few] / (torch.softmax(x, 1) @ values) - 1
+    print(f"mean {off.mean():.2e}, largest {off.abs().max():.2e}")
+    assert off.mean().abs() <= 672 * UNIT + 2.0 ** -13
